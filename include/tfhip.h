@@ -244,6 +244,41 @@ int tfhip_sgemm_fused(int layout, const float* A, const float* B, float* C, size
 int tfhip_sgemm_batched(int layout, const float* A, const float* B, float* C, size_t M, size_t N, size_t K, size_t batch, size_t stride_a, size_t stride_b,
                         size_t stride_c);
 
+/* ---- operators of a training step around the dense layers -----------------------------------------------------
+ * Layer norm, embedding lookup and the orthogonalised update have no node in the reference; its users compose them from
+ * the mean and norm reductions, loads with computed indices and atomic adds (Compiler/Implementations.cpp:243-303,
+ * 451-488), and its optimisers end at the element-wise update (Python/TensorFrost/optimizers.py:104-167). All matrices
+ * are dense row-major fp32; every sum is held in fp32 or wider, in an order that does not change from run to run.
+ * Several host threads may make these calls at once: the launches of one call stay together on the library's stream.
+ * They may be recorded into a graph (run the same work once before, so that the scratch buffer has its size). */
+
+/* y[r,c] = (x[r,c] - mean[r]) * rstd[r] * weight[c] + bias[c], mean[r] = mean_c x[r,:], rstd[r] = 1 / sqrt(mean_c (x[r,:] -
+ * mean[r])^2 + eps). weight and bias may be null (1 and 0). mean and rstd receive the row statistics; each may be null.
+ * x == y (in place) is allowed, any other overlap is refused. rows == 0 is a no-op; cols >= 1; eps finite, >= 0. */
+int tfhip_layer_norm_rows_f32(const float* x, const float* weight, const float* bias, float* y, float* mean, float* rstd, size_t rows, size_t cols, float eps);
+/* With xhat = (x - mean) * rstd and g = dy * weight: dx[r,:] = rstd[r] * (g - mean_c g - xhat * mean_c(g * xhat)),
+ * dweight[c] = sum_r dy * xhat, dbias[c] = sum_r dy. mean and rstd are what the forward call left; weight may be null
+ * (1); each of dx, dweight, dbias may be null, not all three. dx may be x or dy; any other overlap is refused.
+ * rows == 0 leaves zeros in dweight and dbias. */
+int tfhip_layer_norm_rows_backward_f32(const float* x, const float* dy, const float* weight, const float* mean, const float* rstd, float* dx, float* dweight, float* dbias, size_t rows,
+                                       size_t cols);
+
+/* out[i,:] = scale * table[tokens[i],:], i < n. A token outside [0, vocab) (the -1 behind the end of a padded row)
+ * gives a row of zeros. table [vocab, cols], out [n, cols]; vocab, cols >= 1; n == 0 is a no-op; n < 2^30. out may
+ * overlap neither table nor tokens. */
+int tfhip_embedding_rows_f32(const int32_t* tokens, const float* table, float* out, size_t n, size_t vocab, size_t cols, float scale);
+/* dtable[v,:] = scale * sum of dy[i,:] over the i with tokens[i] == v. Every row of dtable is written, rows that no token
+ * names with zeros; tokens outside [0, vocab) contribute nothing. The positions are sorted by token (stable), so the
+ * result is the same from run to run. */
+int tfhip_embedding_rows_backward_f32(const int32_t* tokens, const float* dy, float* dtable, size_t n, size_t vocab, size_t cols, float scale);
+
+/* Orthogonalises `batch` matrices [rows, cols] that follow each other: X = G / (|G|_F + eps), then `steps` times (1 to 64)
+ * A = X X^T, X <- a X + (b A + c A^2) X with that step's three coefficients (host memory, 3 * steps finite floats: a, b, c
+ * of the first step first); with rows > cols the same on the transposed matrix. A matrix of zeros stays zero; one with an infinity or NaN comes out
+ * as NaN. g == out is allowed, any other overlap is refused. At most 32768 on the shorter side, 2^31 - 1
+ * elements in a matrix and 65535 matrices; batch == 0 is a no-op. */
+int tfhip_newton_schulz_f32(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,7 +36,7 @@ def declared_symbols(header: Path | None = None) -> list[str]:
     return sorted(names)
 
 
-_vp, _sz, _u32, _i = C.c_void_p, C.c_size_t, C.c_uint32, C.c_int
+_vp, _sz, _u32, _i, _f = C.c_void_p, C.c_size_t, C.c_uint32, C.c_int, C.c_float
 _SIGNATURES = {
     "tfhip_init": [_i],
     "tfhip_shutdown": [],
@@ -91,6 +91,11 @@ _SIGNATURES = {
     "tfhip_sgemm_tn_colsum": [_vp, _vp, _vp, _vp, _sz, _sz, _sz],
     "tfhip_sgemm_fused": [C.c_int, _vp, _vp, _vp, _sz, _sz, _sz, C.c_int, _vp],
     "tfhip_sgemm_batched": [C.c_int, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz],
+    "tfhip_layer_norm_rows_f32": [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _f],
+    "tfhip_layer_norm_rows_backward_f32": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz],
+    "tfhip_embedding_rows_f32": [_vp, _vp, _vp, _sz, _sz, _sz, _f],
+    "tfhip_embedding_rows_backward_f32": [_vp, _vp, _vp, _sz, _sz, _sz, _f],
+    "tfhip_newton_schulz_f32": [_vp, _vp, _sz, _sz, _sz, _i, C.POINTER(_f), _f],
 }
 for _op in ("sum", "max", "min"):
     for _ax in ("rows", "cols"):

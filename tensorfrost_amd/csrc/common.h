@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "tfhip.h"
 #include "tfhip_test.h"
 
@@ -58,6 +60,9 @@ void* scratch(size_t bytes);
 // up. Returns TFHIP_OK or TFHIP_ERR_HIP with the message recorded.
 int check_async_error();
 
+// What tfhip_radix_sort_kv takes of the scratch arena, from its front, for n keys whose ping-pong buffers the caller gives.
+size_t radix_sort_scratch_bytes(size_t n);
+
 // Finds the device address of the fixed status-word array of the allocation-free scan on `device`, which must be the
 // current device (every GPU holds its own copy at its own address). Called by tfhip_init.
 int locate_static_scratch(int device);
@@ -72,6 +77,42 @@ int locate_static_scratch(int device);
 	do {                                                                                        \
 		if (!::tfhip::state().initialized) return ::tfhip::fail(TFHIP_ERR_STATE, "tfhip_init has not been called"); \
 	} while (0)
+
+// Held by an entry point that issues several launches with the scratch arena between them: a second host thread waits
+// until the launches of the first are on the stream, and the library's device is the current one meanwhile, whatever
+// device the calling thread works on.
+class CallGuard {
+   public:
+	CallGuard() : lock_(mutex()) {
+		if (hipGetDevice(&before_) != hipSuccess) before_ = -1;
+		if (before_ != state().device) ok_ = hipSetDevice(state().device) == hipSuccess;
+	}
+	~CallGuard() {
+		if (before_ >= 0 && before_ != state().device) (void)hipSetDevice(before_);
+	}
+	bool ok() const { return ok_; }
+	CallGuard(const CallGuard&) = delete;
+	CallGuard& operator=(const CallGuard&) = delete;
+
+   private:
+	static std::recursive_mutex& mutex();
+	std::lock_guard<std::recursive_mutex> lock_;
+	int before_ = -1;
+	bool ok_ = true;
+};
+
+#define TFHIP_HOLD_DEVICE()                                                                          \
+	::tfhip::CallGuard _call_guard;                                                                  \
+	do {                                                                                             \
+		if (!_call_guard.ok()) return ::tfhip::fail(TFHIP_ERR_HIP, "the library's device cannot be made current"); \
+	} while (0)
+
+// Whether [a, a + a_words) and [b, b + b_words) share memory; a null pointer shares none.
+inline bool words_overlap(const void* a, size_t a_words, const void* b, size_t b_words) {
+	if (!a || !b) return false;
+	const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+	return pa < pb + b_words * 4 && pb < pa + a_words * 4;
+}
 
 // Checks the launch that was just issued.
 #define TFHIP_CHECK_LAUNCH() TFHIP_CHECK(hipGetLastError())

@@ -358,6 +358,11 @@ __global__ __launch_bounds__(kRsThreads) void radix_onesweep_kernel(
 		radix_onesweep_body<HAS_VALUES, false>(s, tile, keys_in, keys_out, vals_in, vals_out, n, shift, digit_offsets, status, async_error, kind, encode_on_load, decode_on_store);
 }
 
+size_t radix_sort_scratch_bytes(size_t n) {
+	const size_t tiles = (n + kRsTile - 1) / kRsTile;
+	return ((4 * kRadix * 2 + 16 + 4 * tiles * kRadix) * sizeof(uint32_t) + 255) & ~size_t(255);
+}
+
 static int radix_sort_impl(int kind, const uint32_t* keys_in, const uint32_t* vals_in, uint32_t* keys_out, uint32_t* vals_out,
                            uint32_t* keys_tmp, uint32_t* vals_tmp, size_t n) {
 	State& st = state();

@@ -66,6 +66,11 @@ int fail_hip(hipError_t err, const char* what) {
 	return fail(TFHIP_ERR_HIP, "%s failed: %s (%s)", what, hipGetErrorName(err), hipGetErrorString(err));
 }
 
+std::recursive_mutex& CallGuard::mutex() {
+	static std::recursive_mutex m;
+	return m;
+}
+
 void* scratch(size_t bytes) {
 	State& s = state();
 	if (bytes <= s.scratch_bytes) return s.scratch;

@@ -72,6 +72,17 @@ class DeviceBuffer:
         call("tfhip_malloc", C.byref(ptr), n_words)
         self.ptr = ptr.value
         self.n_words = int(n_words)
+        self.owned = True
+
+    @classmethod
+    def view(cls, ptr: int, n_words: int) -> "DeviceBuffer":
+        """A buffer over device memory that something else owns (a tensor of another library): never freed from here.
+        The library's work runs on its own stream, so what fills or reads that memory elsewhere has to be waited for."""
+        if not ptr or ptr % 4 or n_words <= 0:
+            raise ValueError("a view needs a 4-byte aligned device address and at least one word")
+        buf = cls.__new__(cls)
+        buf.ptr, buf.n_words, buf.owned = int(ptr), int(n_words), False
+        return buf
 
     @classmethod
     def from_numpy(cls, arr) -> "DeviceBuffer":
@@ -103,7 +114,8 @@ class DeviceBuffer:
     def free(self) -> None:
         if self.ptr:
             ptr, self.ptr = self.ptr, None  # the memory is gone even when the call reports an earlier kernel's error
-            call("tfhip_free", ptr)
+            if self.owned:
+                call("tfhip_free", ptr)
 
     def __del__(self):
         try:
@@ -287,7 +299,61 @@ def sgemm(layout: str, a: DeviceBuffer, b: DeviceBuffer, c: DeviceBuffer, m: int
         call("tfhip_sgemm_fused", {"nn": 0, "nt": 1, "tn": 2}[layout], a.ptr, b.ptr, c.ptr, m, n, k, _EPILOGUES[epilogue], aux.ptr if aux is not None else None)
 
 
+def _words(buf: DeviceBuffer | None, n_words: int, name: str):
+    """The address of a buffer that has to hold at least n_words; None stays None."""
+    if buf is None:
+        return None
+    if buf.n_words < n_words:
+        raise ValueError(f"{name} holds {buf.n_words} words, {n_words} are needed")
+    return buf.ptr
+
+
+def layer_norm_rows(x: DeviceBuffer, weight: DeviceBuffer | None, bias: DeviceBuffer | None, y: DeviceBuffer, rows: int, cols: int, eps: float = 1e-5,
+                    mean: DeviceBuffer | None = None, rstd: DeviceBuffer | None = None) -> None:
+    """y = (x - mean) * rstd * weight + bias along every row of x[rows, cols]; mean and rstd receive the rows' statistics,
+    which layer_norm_rows_backward takes. weight / bias None: 1 / 0. x may be y."""
+    n = rows * cols
+    call("tfhip_layer_norm_rows_f32", _words(x, n, "x"), _words(weight, cols, "weight"), _words(bias, cols, "bias"), _words(y, n, "y"), _words(mean, rows, "mean"),
+         _words(rstd, rows, "rstd"), rows, cols, eps)
+
+
+def layer_norm_rows_backward(x: DeviceBuffer, dy: DeviceBuffer, weight: DeviceBuffer | None, mean: DeviceBuffer, rstd: DeviceBuffer, rows: int, cols: int,
+                             dx: DeviceBuffer | None = None, dweight: DeviceBuffer | None = None, dbias: DeviceBuffer | None = None) -> None:
+    """The gradients of layer_norm_rows from the upstream gradient dy; any of dx, dweight, dbias that is given. dx may be
+    x or dy."""
+    n = rows * cols
+    call("tfhip_layer_norm_rows_backward_f32", _words(x, n, "x"), _words(dy, n, "dy"), _words(weight, cols, "weight"), _words(mean, rows, "mean"), _words(rstd, rows, "rstd"),
+         _words(dx, n, "dx"), _words(dweight, cols, "dweight"), _words(dbias, cols, "dbias"), rows, cols)
+
+
+def embedding_rows(tokens: DeviceBuffer, table: DeviceBuffer, out: DeviceBuffer, n: int, vocab: int, cols: int, scale: float = 1.0) -> None:
+    """out[i] = scale * table[tokens[i]] for n int32 tokens; zeros for a token outside [0, vocab)."""
+    call("tfhip_embedding_rows_f32", _words(tokens, n, "tokens"), _words(table, vocab * cols, "table"), _words(out, n * cols, "out"), n, vocab, cols, scale)
+
+
+def embedding_rows_backward(tokens: DeviceBuffer, dy: DeviceBuffer, dtable: DeviceBuffer, n: int, vocab: int, cols: int, scale: float = 1.0) -> None:
+    """dtable[v] = scale * the sum of dy[i] over the positions with tokens[i] == v; every row of dtable is written."""
+    call("tfhip_embedding_rows_backward_f32", _words(tokens, n, "tokens"), _words(dy, n * cols, "dy"), _words(dtable, vocab * cols, "dtable"), n, vocab, cols, scale)
+
+
+NEWTON_SCHULZ_QUINTIC = (3.4445, -4.7750, 2.0315)  # drives singular values into about 0.7 .. 1.2 within five steps
+
+
+def newton_schulz(g: DeviceBuffer, out: DeviceBuffer, rows: int, cols: int, steps: int = 5, batch: int = 1, coefficients=NEWTON_SCHULZ_QUINTIC, eps: float = 1e-7) -> None:
+    """Orthogonalises `batch` matrices [rows, cols] by `steps` Newton-Schulz products. coefficients: (a, b, c) of every
+    step, or one such triple per step. g may be out."""
+    triples = np.asarray(coefficients, dtype=np.float32)
+    if triples.ndim == 1:
+        triples = np.tile(triples, (max(0, steps), 1))
+    if triples.shape != (max(0, steps), 3):
+        raise ValueError(f"{steps} steps need three coefficients, or {steps} x 3; got an array of shape {triples.shape}")
+    triples = np.ascontiguousarray(triples)
+    n = batch * rows * cols
+    call("tfhip_newton_schulz_f32", _words(g, n, "g"), _words(out, n, "out"), batch, rows, cols, steps, triples.ctypes.data_as(C.POINTER(C.c_float)), eps)
+
+
 __all__ = [
     "initialize", "shutdown", "device_info", "synchronize", "DeviceBuffer", "Event", "Kernel",
-    "reduce_rows", "reduce_cols", "reduce_cols_slabs", "softmax_rows", "log_softmax_rows", "scan_inclusive", "radix_sort_kv", "sgemm", "TFHipError",
+    "reduce_rows", "reduce_cols", "reduce_cols_slabs", "softmax_rows", "log_softmax_rows", "scan_inclusive", "radix_sort_kv", "sgemm",
+    "layer_norm_rows", "layer_norm_rows_backward", "embedding_rows", "embedding_rows_backward", "newton_schulz", "NEWTON_SCHULZ_QUINTIC", "TFHipError",
 ]
