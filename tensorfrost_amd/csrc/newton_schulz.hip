@@ -1,10 +1,24 @@
 // Orthogonalisation of matrices by Newton-Schulz products, as optimisers apply it to the update of a dense layer:
 //
-//   X = G / (|G|_F + eps);  per step, with its coefficients a, b, c:  A = X X^T,  B = b A + c A^2,  X <- a X + B X
+//   X = G / (|G|_F + eps);  per step, with its coefficients a, b, c:  A = X X^T,  B = a I + b A + c A^2,  X <- B X
 //
-// (the transposed form for a matrix with more rows than columns, so that A is the smaller of the two squares). Each
+// (on the transposed matrix when there are more rows than columns, so that A is the smaller of the two squares). Each
 // singular value s of X becomes a s + b s^3 + c s^5. The reference has no such operation; its optimisers stop at the
 // element-wise update (Python/TensorFrost/optimizers.py:104-167).
+//
+// Number format. The fp32 matrix instructions reach 157 TFLOP/s here, the fp16 ones 2500. So every operand is held as a
+// pair of fp16 numbers in 32 bits, v = (hi + lo) / scale with hi = fp16(v scale), lo = fp16(v scale - hi), and a product is
+// three fp16 products into one fp32 accumulator, hi hi + hi lo + lo hi. The pair keeps 22 bits, one less than fp32 keeps
+// on average, and the dropped lo lo is below 2^-22 of the product; in exchange the accumulator takes 16 terms a step instead of
+// 2, and the result after five steps is as far from the 64-bit one as that of fp32 products (1.3e-6 against 1.6e-6 of the norm at
+// 256 x 256). The scale is a power of two chosen on the host: the spectral norm of X is at most 1 at the start and at most
+// max |a s + b s^3 + c s^5| over the reachable s after a step, and no element exceeds it; the scale puts that bound at 2^15.
+// Elements below 2^-12 of the bound keep an absolute error of 2^-40 of it instead of a relative one.
+//
+// Layout. A row of a split matrix is a sequence of 128-byte blocks, 32 hi then the 32 lo of the same columns, so one
+// cache line holds a row's share of a step of 32 in k. Rows and columns are padded to whole tiles with zeros, which stay
+// zeros through every product: no kernel but the first and the last tests a bound. All products have both operands
+// contiguous along k (row i of P times row j of Q): A and B are symmetric, and X is kept in both orientations.
 
 #include "common.h"
 
@@ -12,77 +26,400 @@
 
 namespace tfhip {
 
-constexpr int kNsTile = 32;
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+
+constexpr int kNsBlock = 128;  // bytes of a row's block: 32 columns, hi and lo
+constexpr int kNsStep = 32;    // columns of a block
+
+// ---- split values --------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t split_pair(float v) {
+	const _Float16 hi = (_Float16)v;
+	const _Float16 lo = (_Float16)(v - (float)hi);
+	return (uint32_t)__builtin_bit_cast(unsigned short, hi) | ((uint32_t)__builtin_bit_cast(unsigned short, lo) << 16);
+}
+
+// One wave writes a 32 x 32 tile of split values that its lanes hold in the layout of a 32 x 32 accumulator (element r of
+// lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32) as 32 whole blocks: `straight` receives rows (block i =
+// row i), `turned` columns (block i = column i); either may be null. `lds` is 32 x 33 words of this wave's own.
+__device__ __forceinline__ void store_split_tile(const float (&v)[16], uint32_t* lds, char* straight, size_t straight_stride, char* turned, size_t turned_stride) {
+	const int lane = threadIdx.x & 63;
+	__builtin_amdgcn_wave_barrier();
+#pragma unroll
+	for (int r = 0; r < 16; r++) lds[(8 * (r / 4) + 4 * (lane >> 5) + r % 4) * 33 + (lane & 31)] = split_pair(v[r]);
+	__builtin_amdgcn_wave_barrier();
+	const int line = lane >> 1, part = lane & 1;  // two lanes a block: 16 of its columns each
+#pragma unroll
+	for (int form = 0; form < 2; form++) {
+		char* to = form == 0 ? straight : turned;
+		if (!to) continue;
+		uint32_t hi[8], lo[8];
+#pragma unroll
+		for (int k = 0; k < 8; k++) {
+			const int c = part * 16 + 2 * k;
+			const uint32_t p = form == 0 ? lds[line * 33 + c] : lds[c * 33 + line];
+			const uint32_t q = form == 0 ? lds[line * 33 + c + 1] : lds[(c + 1) * 33 + line];
+			hi[k] = (p & 0xFFFFu) | (q << 16);
+			lo[k] = (p >> 16) | (q & 0xFFFF0000u);
+		}
+		char* at = to + (size_t)line * (form == 0 ? straight_stride : turned_stride) + part * 32;
+		*reinterpret_cast<uintx4*>(at) = uintx4{hi[0], hi[1], hi[2], hi[3]};
+		*reinterpret_cast<uintx4*>(at + 16) = uintx4{hi[4], hi[5], hi[6], hi[7]};
+		*reinterpret_cast<uintx4*>(at + 64) = uintx4{lo[0], lo[1], lo[2], lo[3]};
+		*reinterpret_cast<uintx4*>(at + 80) = uintx4{lo[4], lo[5], lo[6], lo[7]};
+	}
+}
+
+// ---- the norm and the first split -----------------------------------------------------------------
 
 // Partial sums of squares, in 64 bits: the square of a large fp32 number does not fit fp32.
 __global__ __launch_bounds__(256) void ns_norm_kernel(const float* __restrict__ g, double* __restrict__ partial, size_t elements, unsigned parts) {
-	__shared__ double red[256];
+	__shared__ double red[4];
 	const size_t matrix = blockIdx.x / parts, part = blockIdx.x % parts;
 	const float* p = g + matrix * elements;
 	double sum = 0.0;
 	for (size_t i = part * 256 + threadIdx.x; i < elements; i += (size_t)parts * 256) sum += (double)p[i] * (double)p[i];
-	red[threadIdx.x] = sum;
+	sum = wave_reduce(sum, [](double a, double b) { return a + b; });
+	if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
 	__syncthreads();
-	for (int off = 128; off >= 1; off >>= 1) {
-		if ((int)threadIdx.x < off) red[threadIdx.x] += red[threadIdx.x + off];
-		__syncthreads();
-	}
-	if (threadIdx.x == 0) partial[blockIdx.x] = red[0];
+	if (threadIdx.x == 0) partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// x = g / (norm + eps), x with at most as many rows as columns (transposed: g is [n, m]).
-__global__ __launch_bounds__(256) void ns_scale_kernel(const float* __restrict__ g, const double* __restrict__ partial, unsigned parts, float* __restrict__ x, size_t m, size_t n, bool transposed,
-                                                       float eps, unsigned groups) {
-	const size_t matrix = blockIdx.x / groups;
+// X and its transpose in split form from g. X is [mp, np] with mp, np padded; `transposed`: g is [n, m], else [m, n].
+// A wave per 32 x 32 tile.
+__global__ __launch_bounds__(256) void ns_split_kernel(const float* __restrict__ g, const double* __restrict__ partial, unsigned parts, char* x, char* xt, size_t m, size_t n, size_t mp, size_t np,
+                                                       bool transposed, float eps, float scale) {
+	__shared__ uint32_t lds[4][32 * 33];
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+	const size_t matrix = blockIdx.y, tiles_n = np / 32, tile = (size_t)blockIdx.x * 4 + wave;
+	if (tile >= tiles_n * (mp / 32)) return;
 	double sum = 0.0;
-	for (unsigned k = 0; k < parts; k++) sum += partial[matrix * parts + k];
+	for (unsigned k = lane; k < parts; k += 64) sum += partial[matrix * parts + k];
+	sum = wave_reduce(sum, [](double a, double b) { return a + b; });
 	const double norm = sqrt(sum) + (double)eps;
-	const float r = !isfinite(norm) ? nanf("") : norm > 0.0 ? (float)(1.0 / norm) : 0.0f;
-	for (size_t i = (size_t)(blockIdx.x % groups) * 256 + threadIdx.x; i < m * n; i += (size_t)groups * 256) {
-		const size_t row = i / n, col = i % n;
-		x[matrix * m * n + i] = r * (transposed ? g[matrix * m * n + col * m + row] : g[matrix * m * n + i]);
+	const double r = !isfinite(norm) ? (double)nanf("") : norm > 0.0 ? (double)scale / norm : 0.0;
+	// the tile in the orientation of g, so that its rows are read along memory
+	const size_t t0 = tile / tiles_n * 32, t1 = tile % tiles_n * 32;
+	const size_t rows = transposed ? n : m, cols = transposed ? m : n, r0 = transposed ? t1 : t0, c0 = transposed ? t0 : t1;
+	g += matrix * m * n;
+	float v[16];
+#pragma unroll
+	for (int k = 0; k < 16; k++) {
+		const size_t row = r0 + 8 * (k / 4) + 4 * (lane >> 5) + k % 4, col = c0 + (lane & 31);
+		v[k] = row < rows && col < cols ? (float)((double)g[row * cols + col] * r) : 0.0f;
 	}
+	x += matrix * mp * np * 4 + t0 * np * 4 + t1 * 4;
+	xt += matrix * mp * np * 4 + t1 * mp * 4 + t0 * 4;
+	store_split_tile(v, lds[wave], transposed ? xt : x, transposed ? mp * 4 : np * 4, transposed ? x : xt, transposed ? np * 4 : mp * 4);
 }
 
-// C = alpha P op(Q) + beta D, fp32, a 32 x 32 tile per group of 256 threads. P [M, K]; Q [N, K] (nt) or [K, N].
-template <bool NT>
-__global__ __launch_bounds__(256) void ns_product_kernel(const float* __restrict__ P, const float* __restrict__ Q, const float* __restrict__ D, float* __restrict__ C, size_t M, size_t N, size_t K,
-                                                         float alpha, float beta) {
-	__shared__ float p[kNsTile][kNsTile + 1], q[kNsTile][kNsTile + 1];
-	P += blockIdx.z * M * K;
-	Q += blockIdx.z * N * K;
-	D += blockIdx.z * M * N;
-	C += blockIdx.z * M * N;
-	const size_t m0 = (size_t)blockIdx.y * kNsTile, n0 = (size_t)blockIdx.x * kNsTile;
-	const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-	float acc[4] = {};
-	for (size_t k0 = 0; k0 < K; k0 += kNsTile) {
-		for (int i = ty; i < kNsTile; i += 8) {
-			p[i][tx] = m0 + i < M && k0 + tx < K ? P[(m0 + i) * K + k0 + tx] : 0.0f;
-			if (NT)
-				q[i][tx] = n0 + i < N && k0 + tx < K ? Q[(n0 + i) * K + k0 + tx] : 0.0f;
-			else
-				q[tx][i] = n0 + tx < N && k0 + i < K ? Q[(k0 + i) * N + n0 + tx] : 0.0f;
+// ---- the products ---------------------------------------------------------------------------------
+
+enum NsKind {
+	kNsGram,    // A = X X^T: tiles on and below the diagonal, each written in both orientations
+	kNsPoly,    // B = a I + b A + c A^2: the same tiles
+	kNsUpdate,  // X <- B X, written in both orientations
+	kNsLast     // the same in fp32, into the caller's matrix
+};
+
+struct NsArgs {
+	const char* P;  // tile rows: [p_tiles * TILE, k_blocks * 32]
+	const char* Q;  // tile columns
+	char* straight;  // out[row of P, row of Q]
+	char* turned;    // out[row of Q, row of P]
+	float* out;      // kNsLast: [out_rows, out_cols]
+	size_t batch_p, batch_q, batch_out;        // bytes between the matrices of a batch
+	size_t straight_stride, turned_stride;     // bytes between rows
+	size_t out_rows, out_cols;
+	uint32_t k_blocks;
+	uint32_t tiles_p, tiles_q;
+	float alpha;  // what an element of the accumulator is multiplied with
+	float beta;   // kNsPoly: what an element of A (as stored) is multiplied with
+	float gamma;  // kNsPoly: what is added on the diagonal
+};
+
+__device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
+
+// 16 bytes per lane from base + offset to group memory at `to` + 16 lane. No vector register is written; the data is there
+// after a wait for the vector-memory counter. (m0 is set where it is used: nothing else in these kernels reads it.)
+__device__ __forceinline__ void load_to_lds(uint32_t to, uint32_t offset, const char* base) {
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
+
+// A group of WP x WQ waves owns a TP x TQ tile of the result.
+template <int TP, int TQ, int WP, int WQ, int KIND>
+__global__ __launch_bounds__(WP* WQ * 64) void ns_product_kernel(const NsArgs g) {
+	constexpr int kWaves = WP * WQ;
+	constexpr int kRows = TP + TQ;
+	constexpr int kStage = kRows * kNsBlock;             // bytes of one step of both operands
+	constexpr int kLoads = kRows / (8 * kWaves);         // a load of a wave brings 8 rows
+	constexpr int SP = TP / WP / 32, SQ = TQ / WQ / 32;  // 32 x 32 tiles of a wave
+	static_assert(kLoads * 8 * kWaves == kRows, "rows divide among the waves");
+	static_assert(TP % (8 * kLoads) == 0, "a wave's rows belong to one operand");
+	static_assert(2 * kStage >= kWaves * 32 * 33 * 4, "the write-out fits the panels' memory");
+	__shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+
+	const int lane = threadIdx.x & 63;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	// consecutive groups go to different dies: give each die a run of neighbouring tiles
+	uint32_t t = blockIdx.x;
+	{
+		const uint32_t q = gridDim.x >> 3, rem = gridDim.x & 7, die = t & 7, at = t >> 3;
+		t = die * q + (die < rem ? die : rem) + at;
+	}
+	uint32_t tp, tq;
+	if (KIND == kNsGram || KIND == kNsPoly) {  // row tp of the lower triangle holds tp + 1 tiles
+		tp = (uint32_t)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
+		while (tp * (tp + 1) / 2 > t) tp--;
+		while ((tp + 1) * (tp + 2) / 2 <= t) tp++;
+		tq = t - tp * (tp + 1) / 2;
+	} else {
+		tp = t / g.tiles_q;
+		tq = t - tp * g.tiles_q;
+	}
+	const size_t stride = (size_t)g.k_blocks * kNsBlock;
+	const char* P = g.P + blockIdx.y * g.batch_p + (size_t)tp * TP * stride;
+	const char* Q = g.Q + blockIdx.y * g.batch_q + (size_t)tq * TQ * stride;
+
+	// Row r of a stage lies at 128 r; its 16-byte piece c at place c ^ (r / 2 % 8), so that the 16 lanes that read one
+	// piece of 16 rows together meet 16 different quarters of the banks.
+	const int first_row = wave * kLoads * 8;
+	const char* src = first_row < TP ? P + (size_t)first_row * stride : Q + (size_t)(first_row - TP) * stride;
+	uint32_t offset[kLoads];
+#pragma unroll
+	for (int i = 0; i < kLoads; i++) {
+		const uint32_t row = i * 8 + (lane >> 3);
+		offset[i] = row * (uint32_t)stride + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+	}
+	const uint32_t lds0 = lds_offset(lds) + first_row * kNsBlock;
+
+	floatx16 acc[SP][SQ];
+#pragma unroll
+	for (int i = 0; i < SP; i++)
+#pragma unroll
+		for (int j = 0; j < SQ; j++)
+#pragma unroll
+			for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+
+	const int wp = wave / WQ, wq = wave % WQ;
+	const int swizzle = ((lane & 31) >> 1) & 7;
+	const char* frag_p = lds + (wp * SP * 32 + (lane & 31)) * kNsBlock;
+	const char* frag_q = lds + (TP + wq * SQ * 32 + (lane & 31)) * kNsBlock;
+
+#pragma unroll
+	for (int i = 0; i < kLoads; i++) load_to_lds(lds0 + i * 1024, offset[i], src);
+	for (uint32_t k = 0; k < g.k_blocks; k++) {
+		asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+		__syncthreads();  // this step's panels are there, the other buffer has been read by everyone
+		const uint32_t cur = (k & 1) * kStage;
+		if (k + 1 < g.k_blocks) {
+			src += kNsBlock;
+#pragma unroll
+			for (int i = 0; i < kLoads; i++) load_to_lds(lds0 + (kStage - cur) + i * 1024, offset[i], src);
 		}
-		__syncthreads();
-		for (int k = 0; k < kNsTile; k++)
 #pragma unroll
-			for (int j = 0; j < 4; j++) acc[j] += p[ty + 8 * j][k] * q[tx][k];
-		__syncthreads();
-	}
+		for (int h = 0; h < 2; h++) {
+			const int hi_at = ((2 * h + (lane >> 5)) ^ swizzle) << 4, lo_at = hi_at ^ 64;
+			half8 p_hi[SP], p_lo[SP], q_hi[SQ], q_lo[SQ];
 #pragma unroll
-	for (int j = 0; j < 4; j++) {
-		const size_t row = m0 + ty + 8 * j, col = n0 + tx;
-		if (row < M && col < N) C[row * N + col] = alpha * acc[j] + (beta != 0.0f ? beta * D[row * N + col] : 0.0f);
+			for (int i = 0; i < SP; i++) {
+				p_hi[i] = *reinterpret_cast<const half8*>(frag_p + cur + i * 32 * kNsBlock + hi_at);
+				p_lo[i] = *reinterpret_cast<const half8*>(frag_p + cur + i * 32 * kNsBlock + lo_at);
+			}
+#pragma unroll
+			for (int j = 0; j < SQ; j++) {
+				q_hi[j] = *reinterpret_cast<const half8*>(frag_q + cur + j * 32 * kNsBlock + hi_at);
+				q_lo[j] = *reinterpret_cast<const half8*>(frag_q + cur + j * 32 * kNsBlock + lo_at);
+			}
+#pragma unroll
+			for (int i = 0; i < SP; i++)
+#pragma unroll
+				for (int j = 0; j < SQ; j++) {
+					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_lo[i], q_hi[j], acc[i][j], 0, 0, 0);
+					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi[i], q_lo[j], acc[i][j], 0, 0, 0);
+					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi[i], q_hi[j], acc[i][j], 0, 0, 0);
+				}
+		}
 	}
+	__syncthreads();  // the panels' memory becomes the waves' corners of the write-out
+
+	uint32_t* corner = reinterpret_cast<uint32_t*>(lds) + wave * 32 * 33;
+	const uint32_t p0 = tp * TP + wp * SP * 32, q0 = tq * TQ + wq * SQ * 32;
+#pragma unroll
+	for (int i = 0; i < SP; i++)
+#pragma unroll
+		for (int j = 0; j < SQ; j++) {
+			const uint32_t row0 = p0 + i * 32, col0 = q0 + j * 32;
+			float v[16];
+#pragma unroll
+			for (int r = 0; r < 16; r++) v[r] = g.alpha * acc[i][j][r];
+			if (KIND == kNsPoly) {
+				// A is symmetric: its four rows of a lane are four columns of one row
+				const char* a = P - (size_t)tp * TP * stride + (size_t)(col0 + (lane & 31)) * stride + (size_t)row0 * 4 + 8 * (lane >> 5);
+#pragma unroll
+				for (int q = 0; q < 4; q++) {
+					typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+					const half4 hi = *reinterpret_cast<const half4*>(a + 16 * q), lo = *reinterpret_cast<const half4*>(a + 16 * q + 64);
+#pragma unroll
+					for (int r = 0; r < 4; r++) {
+						v[4 * q + r] += g.beta * ((float)hi[r] + (float)lo[r]);
+						if (row0 + 8 * q + 4 * (lane >> 5) + r == col0 + (lane & 31)) v[4 * q + r] += g.gamma;
+					}
+				}
+			}
+			if (KIND == kNsLast) {
+				float* out = reinterpret_cast<float*>(reinterpret_cast<char*>(g.out) + blockIdx.y * g.batch_out);
+				const size_t col = col0 + (lane & 31);
+#pragma unroll
+				for (int r = 0; r < 16; r++) {
+					const size_t row = row0 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+					if (row < g.out_rows && col < g.out_cols) out[row * g.out_cols + col] = v[r];
+				}
+			} else {
+				char* straight = g.straight + blockIdx.y * g.batch_out + (size_t)row0 * g.straight_stride + (size_t)col0 * 4;
+				char* turned = g.turned + blockIdx.y * g.batch_out + (size_t)col0 * g.turned_stride + (size_t)row0 * 4;
+				// a tile on the diagonal is its own mirror: each of its elements has one writer
+				if ((KIND == kNsGram || KIND == kNsPoly) && tp == tq) turned = nullptr;
+				store_split_tile(v, corner, straight, g.straight_stride, turned, g.turned_stride);
+			}
+		}
 }
 
-__global__ __launch_bounds__(256) void ns_store_kernel(const float* __restrict__ x, float* __restrict__ out, size_t m, size_t n, bool transposed, unsigned groups) {
-	const size_t matrix = blockIdx.x / groups;
-	for (size_t i = (size_t)(blockIdx.x % groups) * 256 + threadIdx.x; i < m * n; i += (size_t)groups * 256) {
-		const size_t row = i / n, col = i % n;
-		out[matrix * m * n + (transposed ? col * m + row : i)] = x[matrix * m * n + i];
+// ---- the host's side --------------------------------------------------------------------------------
+
+// max over s in [0, top] of |a s + b s^3 + c s^5| (odd) or |a + b s^2 + c s^4|: at the ends or where the derivative is 0.
+static double largest(double a, double b, double c, double top, bool odd) {
+	double best = 0.0;
+	auto look = [&](double t) {  // t = s^2
+		if (!(t >= 0.0 && t <= top * top)) return;
+		const double p = fabs((a + t * (b + t * c)) * (odd ? sqrt(t) : 1.0));
+		if (!(p <= best)) best = p;
+	};
+	look(0.0);
+	look(top * top);
+	const double u = odd ? a : b, v = odd ? 3.0 * b : 2.0 * c, w = odd ? 5.0 * c : 0.0;  // u + v t + w t^2 = 0
+	if (w == 0.0) {
+		if (v != 0.0) look(-u / v);
+	} else {
+		const double d = v * v - 4.0 * u * w;
+		if (d >= 0.0) {
+			look((-v + sqrt(d)) / (2.0 * w));
+			look((-v - sqrt(d)) / (2.0 * w));
+		}
 	}
+	return best;
+}
+
+// The power of two that brings values of at most `bound` to at most 2^15.
+static double scale_for(double bound) {
+	if (!(bound > 1e-18)) bound = 1e-18;
+	if (!(bound < 1e18)) bound = 1e18;
+	int e;
+	frexp(bound, &e);  // bound <= 2^e
+	return ldexp(1.0, 15 - e);
+}
+
+template <int KIND>
+static int ns_product(const NsArgs& a, int tile, size_t batch) {
+	const bool half = KIND == kNsGram || KIND == kNsPoly;
+	const unsigned tiles = half ? a.tiles_p * (a.tiles_p + 1) / 2 : a.tiles_p * a.tiles_q;
+	const dim3 grid(tiles, (unsigned)batch);
+	if (tile == 128)
+		hipLaunchKernelGGL((ns_product_kernel<128, 128, 2, 2, KIND>), grid, dim3(256), 0, state().stream, a);
+	else
+		hipLaunchKernelGGL((ns_product_kernel<64, 64, 2, 2, KIND>), grid, dim3(256), 0, state().stream, a);
+	TFHIP_CHECK_LAUNCH();
+	return TFHIP_OK;
+}
+
+static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps) {
+	State& s = state();
+	const bool transposed = rows > cols;
+	const size_t m = transposed ? cols : rows, n = transposed ? rows : cols, elements = rows * cols;
+	const int tile = m > 512 ? 128 : 64;
+	const size_t mp = (m + tile - 1) / tile * tile, np = (n + tile - 1) / tile * tile;
+	const unsigned parts = (unsigned)(elements < 4096 ? 1 : elements / 4096 < 256 ? elements / 4096 : 256);
+	auto align = [](size_t b) { return (b + 255) & ~size_t(255); };
+	const size_t norm_bytes = align(batch * parts * sizeof(double)), x_bytes = align(batch * mp * np * 4), a_bytes = align(batch * mp * mp * 4);
+	char* base = (char*)scratch(norm_bytes + 4 * x_bytes + 2 * a_bytes);
+	if (!base) return TFHIP_ERR_HIP;
+	double* partial = (double*)base;
+	char* x = base + norm_bytes;
+	char* xt = x + x_bytes;
+	char* x_next = xt + x_bytes;
+	char* xt_next = x_next + x_bytes;
+	char* A = xt_next + x_bytes;
+	char* B = A + a_bytes;
+
+	hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)batch * parts), dim3(256), 0, s.stream, g, partial, elements, parts);
+	TFHIP_CHECK_LAUNCH();
+	double bound = 1.0;
+	double scale_x = scale_for(bound);
+	hipLaunchKernelGGL(ns_split_kernel, dim3((unsigned)((mp / 32 * (np / 32) + 3) / 4), (unsigned)batch), dim3(256), 0, s.stream, g, (const double*)partial, parts, x, xt, m, n, mp, np, transposed, eps,
+	                   (float)scale_x);
+	TFHIP_CHECK_LAUNCH();
+	for (int k = 0; k < steps; k++) {
+		const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
+		// a bound that rounding does not cross
+		const double scale_a = scale_for(bound * bound * 1.0001), scale_b = scale_for(largest(a, b, c, bound, false) * 1.0001);
+		const double next = largest(a, b, c, bound, true) * 1.0001, scale_next = scale_for(next);
+		NsArgs args = {};
+		args.P = args.Q = x;
+		args.straight = args.turned = A;
+		args.straight_stride = args.turned_stride = mp * 4;
+		args.batch_p = args.batch_q = mp * np * 4;
+		args.batch_out = mp * mp * 4;
+		args.k_blocks = (uint32_t)(np / kNsStep);
+		args.tiles_p = args.tiles_q = (uint32_t)(mp / tile);
+		args.alpha = (float)(scale_a / (scale_x * scale_x));
+		int rc = ns_product<kNsGram>(args, tile, batch);
+		if (rc) return rc;
+		args.P = args.Q = A;
+		args.straight = args.turned = B;
+		args.batch_p = args.batch_q = mp * mp * 4;
+		args.k_blocks = (uint32_t)(mp / kNsStep);
+		args.alpha = (float)(c * scale_b / (scale_a * scale_a));
+		args.beta = (float)(b * scale_b / scale_a);
+		args.gamma = (float)(a * scale_b);
+		rc = ns_product<kNsPoly>(args, tile, batch);
+		if (rc) return rc;
+		const bool last = k + 1 == steps;
+		const bool turn = last && transposed;  // the caller's rows are the columns of X
+		args.P = turn ? xt : B;
+		args.Q = turn ? B : xt;
+		args.batch_p = turn ? mp * np * 4 : mp * mp * 4;
+		args.batch_q = turn ? mp * mp * 4 : mp * np * 4;
+		args.tiles_p = (uint32_t)((turn ? np : mp) / tile);
+		args.tiles_q = (uint32_t)((turn ? mp : np) / tile);
+		if (last) {
+			args.out = out;
+			args.out_rows = rows;
+			args.out_cols = cols;
+			args.batch_out = elements * sizeof(float);
+			args.alpha = (float)(1.0 / (scale_b * scale_x));
+			rc = ns_product<kNsLast>(args, tile, batch);
+		} else {
+			args.straight = x_next;
+			args.turned = xt_next;
+			args.straight_stride = np * 4;
+			args.turned_stride = mp * 4;
+			args.batch_out = mp * np * 4;
+			args.alpha = (float)(scale_next / (scale_b * scale_x));
+			rc = ns_product<kNsUpdate>(args, tile, batch);
+		}
+		if (rc) return rc;
+		char* t = x;
+		x = x_next;
+		x_next = t;
+		t = xt;
+		xt = xt_next;
+		xt_next = t;
+		bound = next;
+		scale_x = scale_next;
+	}
+	return TFHIP_OK;
 }
 
 }  // namespace tfhip
@@ -91,10 +428,9 @@ using namespace tfhip;
 
 extern "C" int tfhip_newton_schulz_f32(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps) {
 	if (rows == 0 || cols == 0) return fail(TFHIP_ERR_ARG, "orthogonalisation of an empty matrix (%zu x %zu)", rows, cols);
-	if (rows > 32768 || cols > 0x7FFFFF || cols * rows > 0x7FFFFFFF) {
-		if (cols > 32768 || rows > 0x7FFFFF || cols * rows > 0x7FFFFFFF)
-			return fail(TFHIP_ERR_ARG, "orthogonalisation of a %zu x %zu matrix: at most 32768 on its shorter side and 2^31 - 1 elements", rows, cols);
-	}
+	const size_t shorter = rows < cols ? rows : cols, longer = rows < cols ? cols : rows;
+	if (shorter > 32768 || longer > 0x7FFFFF || rows * cols > 0x7FFFFFFF)
+		return fail(TFHIP_ERR_ARG, "orthogonalisation of a %zu x %zu matrix: at most 32768 on its shorter side, 2^23 - 1 on its longer one and 2^31 - 1 elements", rows, cols);
 	if (batch > 65535) return fail(TFHIP_ERR_ARG, "more than 65535 matrices in one batch (%zu)", batch);
 	if (steps < 1 || steps > 64) return fail(TFHIP_ERR_ARG, "%d Newton-Schulz steps (1 to 64 are taken)", steps);
 	if (!coefficients) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_newton_schulz_f32");
@@ -103,42 +439,8 @@ extern "C" int tfhip_newton_schulz_f32(const float* g, float* out, size_t batch,
 	if (!(eps >= 0.0f) || !isfinite(eps)) return fail(TFHIP_ERR_ARG, "Newton-Schulz with eps = %g: a finite number of at least 0 is needed", (double)eps);
 	if (batch == 0) return TFHIP_OK;
 	if (!g || !out) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_newton_schulz_f32");
-	const size_t elements = rows * cols;
-	if (g != out && words_overlap(g, batch * elements, out, batch * elements)) return fail(TFHIP_ERR_ARG, "Newton-Schulz: g and out overlap without being the same");
+	if (g != out && words_overlap(g, batch * rows * cols, out, batch * rows * cols)) return fail(TFHIP_ERR_ARG, "Newton-Schulz: g and out overlap without being the same");
 	TFHIP_REQUIRE_INIT();
 	TFHIP_HOLD_DEVICE();
-	State& s = state();
-	const bool transposed = rows > cols;
-	const size_t m = transposed ? cols : rows, n = transposed ? rows : cols;
-	const unsigned parts = (unsigned)(elements < 4096 ? 1 : elements / 4096 < 256 ? elements / 4096 : 256);
-	const size_t norm_bytes = (batch * parts * sizeof(double) + 255) & ~size_t(255);
-	const size_t x_bytes = (batch * elements * sizeof(float) + 255) & ~size_t(255), a_bytes = (batch * m * m * sizeof(float) + 255) & ~size_t(255);
-	char* base = (char*)scratch(norm_bytes + 2 * x_bytes + 2 * a_bytes);
-	if (!base) return TFHIP_ERR_HIP;
-	double* partial = (double*)base;
-	float* x = (float*)(base + norm_bytes);
-	float* x2 = (float*)(base + norm_bytes + x_bytes);
-	float* A = (float*)(base + norm_bytes + 2 * x_bytes);
-	float* B = (float*)(base + norm_bytes + 2 * x_bytes + a_bytes);
-	const unsigned groups = (unsigned)(elements / 1024 + 1 < 1024 ? elements / 1024 + 1 : 1024);
-	hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)batch * parts), dim3(256), 0, s.stream, g, partial, elements, parts);
-	TFHIP_CHECK_LAUNCH();
-	hipLaunchKernelGGL(ns_scale_kernel, dim3((unsigned)batch * groups), dim3(256), 0, s.stream, g, (const double*)partial, parts, x, m, n, transposed, eps, groups);
-	TFHIP_CHECK_LAUNCH();
-	const unsigned mt = (unsigned)((m + kNsTile - 1) / kNsTile), nt = (unsigned)((n + kNsTile - 1) / kNsTile);
-	for (int k = 0; k < steps; k++) {
-		const float a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
-		hipLaunchKernelGGL(ns_product_kernel<true>, dim3(mt, mt, (unsigned)batch), dim3(256), 0, s.stream, x, x, A, A, m, m, n, 1.0f, 0.0f);
-		TFHIP_CHECK_LAUNCH();
-		hipLaunchKernelGGL(ns_product_kernel<true>, dim3(mt, mt, (unsigned)batch), dim3(256), 0, s.stream, A, A, A, B, m, m, m, c, b);
-		TFHIP_CHECK_LAUNCH();
-		hipLaunchKernelGGL(ns_product_kernel<false>, dim3(nt, mt, (unsigned)batch), dim3(256), 0, s.stream, B, x, x, x2, m, n, m, 1.0f, a);
-		TFHIP_CHECK_LAUNCH();
-		float* t = x;
-		x = x2;
-		x2 = t;
-	}
-	hipLaunchKernelGGL(ns_store_kernel, dim3((unsigned)batch * groups), dim3(256), 0, s.stream, (const float*)x, out, m, n, transposed, groups);
-	TFHIP_CHECK_LAUNCH();
-	return TFHIP_OK;
+	return newton_schulz(g, out, batch, rows, cols, steps, coefficients, eps);
 }
