@@ -1,6 +1,6 @@
 // Orthogonalisation of matrices by Newton-Schulz products, as optimisers apply it to the update of a dense layer:
 //
-//   X = G / (|G|_F + eps);  per step, with its coefficients a, b, c:  A = X X^T,  B = a I + b A + c A^2,  X <- B X
+//   X = G / (|G|_F + eps);  per step, with its coefficients a, b, c:  A = X X^T,  B = b A + c A^2,  X <- a X + B X
 //
 // (on the transposed matrix when there are more rows than columns, so that A is the smaller of the two squares). Each
 // singular value s of X becomes a s + b s^3 + c s^5. The reference has no such operation; its optimisers stop at the
@@ -27,6 +27,7 @@
 namespace tfhip {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
@@ -119,25 +120,25 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const float* __restrict__
 
 enum NsKind {
 	kNsGram,    // A = X X^T: tiles on and below the diagonal, each written in both orientations
-	kNsPoly,    // B = a I + b A + c A^2: the same tiles
-	kNsUpdate,  // X <- B X, written in both orientations
+	kNsPoly,    // B = b A + c A^2: the same tiles
+	kNsUpdate,  // X <- a X + B X, written in both orientations
 	kNsLast     // the same in fp32, into the caller's matrix
 };
 
 struct NsArgs {
 	const char* P;  // tile rows: [p_tiles * TILE, k_blocks * 32]
 	const char* Q;  // tile columns
+	const char* addend;  // all but kNsGram: a matrix to add, as [row of Q, row of P]
 	char* straight;  // out[row of P, row of Q]
 	char* turned;    // out[row of Q, row of P]
 	float* out;      // kNsLast: [out_rows, out_cols]
-	size_t batch_p, batch_q, batch_out;        // bytes between the matrices of a batch
-	size_t straight_stride, turned_stride;     // bytes between rows
+	size_t batch_p, batch_q, batch_addend, batch_out;          // bytes between the matrices of a batch
+	size_t addend_stride, straight_stride, turned_stride;      // bytes between rows
 	size_t out_rows, out_cols;
 	uint32_t k_blocks;
 	uint32_t tiles_p, tiles_q;
 	float alpha;  // what an element of the accumulator is multiplied with
-	float beta;   // kNsPoly: what an element of A (as stored) is multiplied with
-	float gamma;  // kNsPoly: what is added on the diagonal
+	float beta;   // ... and an element of the addend
 };
 
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
@@ -255,18 +256,14 @@ __global__ __launch_bounds__(WP* WQ * 64) void ns_product_kernel(const NsArgs g)
 			float v[16];
 #pragma unroll
 			for (int r = 0; r < 16; r++) v[r] = g.alpha * acc[i][j][r];
-			if (KIND == kNsPoly) {
-				// A is symmetric: its four rows of a lane are four columns of one row
-				const char* a = P - (size_t)tp * TP * stride + (size_t)(col0 + (lane & 31)) * stride + (size_t)row0 * 4 + 8 * (lane >> 5);
+			if (KIND != kNsGram) {
+				// stored turned, so that the four rows of a lane are four neighbours
+				const char* a = g.addend + blockIdx.y * g.batch_addend + (size_t)(col0 + (lane & 31)) * g.addend_stride + (size_t)row0 * 4 + 8 * (lane >> 5);
 #pragma unroll
 				for (int q = 0; q < 4; q++) {
-					typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 					const half4 hi = *reinterpret_cast<const half4*>(a + 16 * q), lo = *reinterpret_cast<const half4*>(a + 16 * q + 64);
 #pragma unroll
-					for (int r = 0; r < 4; r++) {
-						v[4 * q + r] += g.beta * ((float)hi[r] + (float)lo[r]);
-						if (row0 + 8 * q + 4 * (lane >> 5) + r == col0 + (lane & 31)) v[4 * q + r] += g.gamma;
-					}
+					for (int r = 0; r < 4; r++) v[4 * q + r] += g.beta * ((float)hi[r] + (float)lo[r]);
 				}
 			}
 			if (KIND == kNsLast) {
@@ -289,27 +286,31 @@ __global__ __launch_bounds__(WP* WQ * 64) void ns_product_kernel(const NsArgs g)
 
 // ---- the host's side --------------------------------------------------------------------------------
 
-// max over s in [0, top] of |a s + b s^3 + c s^5| (odd) or |a + b s^2 + c s^4|: at the ends or where the derivative is 0.
-static double largest(double a, double b, double c, double top, bool odd) {
+// max |a s + b s^3 + c s^5| over s in [0, top]: at the end or where the derivative is 0.
+static double largest_quintic(double a, double b, double c, double top) {
 	double best = 0.0;
 	auto look = [&](double t) {  // t = s^2
 		if (!(t >= 0.0 && t <= top * top)) return;
-		const double p = fabs((a + t * (b + t * c)) * (odd ? sqrt(t) : 1.0));
+		const double p = fabs((a + t * (b + t * c)) * sqrt(t));
 		if (!(p <= best)) best = p;
 	};
-	look(0.0);
 	look(top * top);
-	const double u = odd ? a : b, v = odd ? 3.0 * b : 2.0 * c, w = odd ? 5.0 * c : 0.0;  // u + v t + w t^2 = 0
+	const double u = a, v = 3.0 * b, w = 5.0 * c;  // u + v t + w t^2 = 0
 	if (w == 0.0) {
 		if (v != 0.0) look(-u / v);
-	} else {
-		const double d = v * v - 4.0 * u * w;
-		if (d >= 0.0) {
-			look((-v + sqrt(d)) / (2.0 * w));
-			look((-v - sqrt(d)) / (2.0 * w));
-		}
+	} else if (v * v - 4.0 * u * w >= 0.0) {
+		const double root = sqrt(v * v - 4.0 * u * w);
+		look((-v + root) / (2.0 * w));
+		look((-v - root) / (2.0 * w));
 	}
 	return best;
+}
+
+// max |b t + c t^2| over t in [0, top], likewise.
+static double largest_square(double b, double c, double top) {
+	const double end = fabs(top * (b + top * c)), t = c != 0.0 ? -b / (2.0 * c) : -1.0;
+	const double middle = t > 0.0 && t < top ? fabs(t * (b + t * c)) : 0.0;
+	return end > middle ? end : middle;
 }
 
 // The power of two that brings values of at most `bound` to at most 2^15.
@@ -363,8 +364,8 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 	for (int k = 0; k < steps; k++) {
 		const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
 		// a bound that rounding does not cross
-		const double scale_a = scale_for(bound * bound * 1.0001), scale_b = scale_for(largest(a, b, c, bound, false) * 1.0001);
-		const double next = largest(a, b, c, bound, true) * 1.0001, scale_next = scale_for(next);
+		const double scale_a = scale_for(bound * bound * 1.0001), scale_b = scale_for(largest_square(b, c, bound * bound) * 1.0001);
+		const double next = largest_quintic(a, b, c, bound) * 1.0001, scale_next = scale_for(next);
 		NsArgs args = {};
 		args.P = args.Q = x;
 		args.straight = args.turned = A;
@@ -382,7 +383,9 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 		args.k_blocks = (uint32_t)(mp / kNsStep);
 		args.alpha = (float)(c * scale_b / (scale_a * scale_a));
 		args.beta = (float)(b * scale_b / scale_a);
-		args.gamma = (float)(a * scale_b);
+		args.addend = A;
+		args.addend_stride = mp * 4;
+		args.batch_addend = mp * mp * 4;
 		rc = ns_product<kNsPoly>(args, tile, batch);
 		if (rc) return rc;
 		const bool last = k + 1 == steps;
@@ -391,6 +394,9 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 		args.Q = turn ? B : xt;
 		args.batch_p = turn ? mp * np * 4 : mp * mp * 4;
 		args.batch_q = turn ? mp * mp * 4 : mp * np * 4;
+		args.addend = turn ? x : xt;
+		args.addend_stride = (turn ? np : mp) * 4;
+		args.batch_addend = mp * np * 4;
 		args.tiles_p = (uint32_t)((turn ? np : mp) / tile);
 		args.tiles_q = (uint32_t)((turn ? mp : np) / tile);
 		if (last) {
@@ -399,6 +405,7 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 			args.out_cols = cols;
 			args.batch_out = elements * sizeof(float);
 			args.alpha = (float)(1.0 / (scale_b * scale_x));
+			args.beta = (float)(a / scale_x);
 			rc = ns_product<kNsLast>(args, tile, batch);
 		} else {
 			args.straight = x_next;
@@ -407,6 +414,7 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 			args.turned_stride = mp * 4;
 			args.batch_out = mp * np * 4;
 			args.alpha = (float)(scale_next / (scale_b * scale_x));
+			args.beta = (float)(a * scale_next / scale_x);
 			rc = ns_product<kNsUpdate>(args, tile, batch);
 		}
 		if (rc) return rc;
