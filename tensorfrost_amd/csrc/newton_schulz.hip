@@ -75,45 +75,80 @@ __device__ __forceinline__ void store_split_tile(const float (&v)[16], uint32_t*
 
 // ---- the norm and the first split -----------------------------------------------------------------
 
-// Partial sums of squares, in 64 bits: the square of a large fp32 number does not fit fp32.
-__global__ __launch_bounds__(256) void ns_norm_kernel(const float* __restrict__ g, double* __restrict__ partial, size_t elements, unsigned parts) {
+// Partial sums of squares, in 64 bits: the square of a large fp32 number does not fit fp32. `vec`: every matrix starts on
+// 16 bytes and holds whole vectors. (4096 x 4096: 64 MiB.)
+__global__ __launch_bounds__(256) void ns_norm_kernel(const float* __restrict__ g, double* __restrict__ partial, size_t elements, unsigned parts, bool vec) {
 	__shared__ double red[4];
 	const size_t matrix = blockIdx.x / parts, part = blockIdx.x % parts;
 	const float* p = g + matrix * elements;
-	double sum = 0.0;
-	for (size_t i = part * 256 + threadIdx.x; i < elements; i += (size_t)parts * 256) sum += (double)p[i] * (double)p[i];
-	sum = wave_reduce(sum, [](double a, double b) { return a + b; });
+	double sum = 0.0, sum2 = 0.0;
+	if (vec) {
+		const size_t vecs = elements / 4, step = (size_t)parts * 256;
+		const float4* v = reinterpret_cast<const float4*>(p);
+		size_t i = part * 256 + threadIdx.x;
+		for (; i + 3 * step < vecs; i += 4 * step) {
+			float4 t[4];
+#pragma unroll
+			for (int u = 0; u < 4; u++) t[u] = v[i + u * step];
+#pragma unroll
+			for (int u = 0; u < 4; u++) {
+				sum += (double)t[u].x * (double)t[u].x + (double)t[u].y * (double)t[u].y;
+				sum2 += (double)t[u].z * (double)t[u].z + (double)t[u].w * (double)t[u].w;
+			}
+		}
+		for (; i < vecs; i += step) {
+			const float4 t = v[i];
+			sum += (double)t.x * (double)t.x + (double)t.y * (double)t.y;
+			sum2 += (double)t.z * (double)t.z + (double)t.w * (double)t.w;
+		}
+	} else {
+		for (size_t i = part * 256 + threadIdx.x; i < elements; i += (size_t)parts * 256) sum += (double)p[i] * (double)p[i];
+	}
+	sum = wave_reduce(sum + sum2, [](double a, double b) { return a + b; });
 	if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
 	__syncthreads();
 	if (threadIdx.x == 0) partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // X and its transpose in split form from g. X is [mp, np] with mp, np padded; `transposed`: g is [n, m], else [m, n].
-// A wave per 32 x 32 tile.
+// A wave per 32 x 32 tile, taken in turn; each group adds up the norm's parts for itself once.
 __global__ __launch_bounds__(256) void ns_split_kernel(const float* __restrict__ g, const double* __restrict__ partial, unsigned parts, char* x, char* xt, size_t m, size_t n, size_t mp, size_t np,
                                                        bool transposed, float eps, float scale) {
 	__shared__ uint32_t lds[4][32 * 33];
+	__shared__ double red[4];
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-	const size_t matrix = blockIdx.y, tiles_n = np / 32, tile = (size_t)blockIdx.x * 4 + wave;
-	if (tile >= tiles_n * (mp / 32)) return;
-	double sum = 0.0;
-	for (unsigned k = lane; k < parts; k += 64) sum += partial[matrix * parts + k];
-	sum = wave_reduce(sum, [](double a, double b) { return a + b; });
-	const double norm = sqrt(sum) + (double)eps;
-	const double r = !isfinite(norm) ? (double)nanf("") : norm > 0.0 ? (double)scale / norm : 0.0;
-	// the tile in the orientation of g, so that its rows are read along memory
-	const size_t t0 = tile / tiles_n * 32, t1 = tile % tiles_n * 32;
-	const size_t rows = transposed ? n : m, cols = transposed ? m : n, r0 = transposed ? t1 : t0, c0 = transposed ? t0 : t1;
+	const size_t matrix = blockIdx.y, tiles_n = np / 32, tiles = tiles_n * (mp / 32), step = (size_t)gridDim.x * 4;
+	// tiles in the orientation of g, so that its rows are read along memory
+	const size_t rows = transposed ? n : m, cols = transposed ? m : n;
 	g += matrix * m * n;
 	float v[16];
+	auto load = [&](size_t tile) {
+		const size_t t0 = tile / tiles_n * 32, t1 = tile % tiles_n * 32, r0 = transposed ? t1 : t0, c0 = transposed ? t0 : t1;
 #pragma unroll
-	for (int k = 0; k < 16; k++) {
-		const size_t row = r0 + 8 * (k / 4) + 4 * (lane >> 5) + k % 4, col = c0 + (lane & 31);
-		v[k] = row < rows && col < cols ? (float)((double)g[row * cols + col] * r) : 0.0f;
+		for (int k = 0; k < 16; k++) {
+			const size_t row = r0 + 8 * (k / 4) + 4 * (lane >> 5) + k % 4, col = c0 + (lane & 31);
+			v[k] = row < rows && col < cols ? g[row * cols + col] : 0.0f;
+		}
+	};
+	size_t tile = (size_t)blockIdx.x * 4 + wave;
+	if (tile < tiles) load(tile);
+	double sum = 0.0;
+	for (unsigned k = threadIdx.x; k < parts; k += 256) sum += partial[matrix * parts + k];
+	sum = wave_reduce(sum, [](double a, double b) { return a + b; });
+	if (lane == 0) red[wave] = sum;
+	__syncthreads();
+	const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3])) + (double)eps;
+	const double r = !isfinite(norm) ? (double)nanf("") : norm > 0.0 ? (double)scale / norm : 0.0;
+	while (tile < tiles) {
+		const size_t t0 = tile / tiles_n * 32, t1 = tile % tiles_n * 32;
+#pragma unroll
+		for (int k = 0; k < 16; k++) v[k] = (float)((double)v[k] * r);
+		char* to_x = x + matrix * mp * np * 4 + t0 * np * 4 + t1 * 4;
+		char* to_xt = xt + matrix * mp * np * 4 + t1 * mp * 4 + t0 * 4;
+		store_split_tile(v, lds[wave], transposed ? to_xt : to_x, transposed ? mp * 4 : np * 4, transposed ? to_x : to_xt, transposed ? np * 4 : mp * 4);
+		tile += step;
+		if (tile < tiles) load(tile);
 	}
-	x += matrix * mp * np * 4 + t0 * np * 4 + t1 * 4;
-	xt += matrix * mp * np * 4 + t1 * mp * 4 + t0 * 4;
-	store_split_tile(v, lds[wave], transposed ? xt : x, transposed ? mp * 4 : np * 4, transposed ? x : xt, transposed ? np * 4 : mp * 4);
 }
 
 // ---- the products ---------------------------------------------------------------------------------
@@ -135,8 +170,9 @@ struct NsArgs {
 	size_t batch_p, batch_q, batch_addend, batch_out;          // bytes between the matrices of a batch
 	size_t addend_stride, straight_stride, turned_stride;      // bytes between rows
 	size_t out_rows, out_cols;
-	uint32_t k_blocks;
+	uint32_t k_blocks;          // blocks of a row of P and Q
 	uint32_t tiles_p, tiles_q;
+	uint32_t band;  // tile rows of a patch
 	float alpha;  // what an element of the accumulator is multiplied with
 	float beta;   // ... and an element of the addend
 };
@@ -149,37 +185,101 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, uint32_t offset, const 
 	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
 }
 
+template <int LEFT>
+__device__ __forceinline__ void wait_loads() {
+	static_assert(LEFT >= 0 && LEFT < 64, "the counter has six bits");
+	asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+}
+
+// Which tile of the result a group works on. Consecutive groups go to different dies, each with its own L2: die d gets the
+// d-th run of tiles, and a run fills a compact patch of the result (bands of `band` tile rows, walked down each column of
+// the band before the next), so that a die reads as few different rows of P and Q as its share of the work allows.
+// The symmetric products list each pair of tile rows once as (r, r + c modulo n), c = 0 .. n / 2 (for even n only half of
+// the r at c = n / 2), which makes the triangle a rectangle of n rows.
+template <int KIND>
+__device__ __forceinline__ void tile_of_group(const NsArgs& g, uint32_t& tp, uint32_t& tq) {
+	constexpr bool kHalf = KIND == kNsGram || KIND == kNsPoly;
+	const uint32_t q = gridDim.x >> 3, rem = gridDim.x & 7, die = blockIdx.x & 7;
+	const uint32_t t = die * q + (die < rem ? die : rem) + (blockIdx.x >> 3);
+	const uint32_t rows = g.tiles_p, cols = kHalf ? (g.tiles_p + 1) / 2 : g.tiles_q;
+	uint32_t r, c;
+	if (!kHalf || t < rows * cols) {
+		const uint32_t top = t / (g.band * cols) * g.band, height = rows - top < g.band ? rows - top : g.band, at = t - top * cols;
+		c = at / height;
+		r = top + at - c * height;
+	} else {
+		c = cols;
+		r = t - rows * cols;
+	}
+	if (kHalf) {
+		c = r + c < rows ? r + c : r + c - rows;
+		tp = r > c ? r : c;
+		tq = r > c ? c : r;
+	} else {
+		tp = r;
+		tq = c;
+	}
+}
+
+// The 32 x 32 tile of the addend at (row0, col0) of the result. It is stored turned, so that the four rows of a lane are
+// four neighbours in memory.
+struct Addend {
+	half4 hi[4], lo[4];
+};
+__device__ __forceinline__ void load_addend(const NsArgs& g, Addend& a, uint32_t row0, uint32_t col0) {
+	const int lane = threadIdx.x & 63;
+	const char* p = g.addend + blockIdx.y * g.batch_addend + (size_t)(col0 + (lane & 31)) * g.addend_stride + (size_t)row0 * 4 + 8 * (lane >> 5);
+#pragma unroll
+	for (int q = 0; q < 4; q++) {
+		a.hi[q] = *reinterpret_cast<const half4*>(p + 16 * q);
+		a.lo[q] = *reinterpret_cast<const half4*>(p + 16 * q + 64);
+	}
+}
+
+// What a kind does with a finished 32 x 32 tile of P Q^T at (row0, col0), held by one wave in accumulator layout.
+template <int KIND>
+__device__ __forceinline__ void finish_tile(const NsArgs& g, float (&v)[16], const Addend& a, uint32_t row0, uint32_t col0, bool diagonal, uint32_t* corner) {
+	const int lane = threadIdx.x & 63;
+#pragma unroll
+	for (int r = 0; r < 16; r++) v[r] *= g.alpha;
+	if (KIND != kNsGram) {
+#pragma unroll
+		for (int r = 0; r < 16; r++) v[r] += g.beta * ((float)a.hi[r / 4][r % 4] + (float)a.lo[r / 4][r % 4]);
+	}
+	if (KIND == kNsLast) {
+		float* out = reinterpret_cast<float*>(reinterpret_cast<char*>(g.out) + blockIdx.y * g.batch_out);
+		const size_t col = col0 + (lane & 31);
+#pragma unroll
+		for (int r = 0; r < 16; r++) {
+			const size_t row = row0 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+			if (row < g.out_rows && col < g.out_cols) out[row * g.out_cols + col] = v[r];
+		}
+	} else {
+		char* straight = g.straight + blockIdx.y * g.batch_out + (size_t)row0 * g.straight_stride + (size_t)col0 * 4;
+		char* turned = g.turned + blockIdx.y * g.batch_out + (size_t)col0 * g.turned_stride + (size_t)row0 * 4;
+		// a tile on the diagonal is its own mirror: each of its elements has one writer
+		if ((KIND == kNsGram || KIND == kNsPoly) && diagonal) turned = nullptr;
+		store_split_tile(v, corner, straight, g.straight_stride, turned, g.turned_stride);
+	}
+}
+
 // A group of WP x WQ waves owns a TP x TQ tile of the result.
-template <int TP, int TQ, int WP, int WQ, int KIND>
+template <int TP, int TQ, int WP, int WQ, int STAGES, int KIND>
 __global__ __launch_bounds__(WP* WQ * 64) void ns_product_kernel(const NsArgs g) {
 	constexpr int kWaves = WP * WQ;
 	constexpr int kRows = TP + TQ;
-	constexpr int kStage = kRows * kNsBlock;             // bytes of one step of both operands
+	constexpr int kStage = kRows * kNsBlock;             // bytes of one block of columns of both operands
 	constexpr int kLoads = kRows / (8 * kWaves);         // a load of a wave brings 8 rows
 	constexpr int SP = TP / WP / 32, SQ = TQ / WQ / 32;  // 32 x 32 tiles of a wave
 	static_assert(kLoads * 8 * kWaves == kRows, "rows divide among the waves");
 	static_assert(TP % (8 * kLoads) == 0, "a wave's rows belong to one operand");
-	static_assert(2 * kStage >= kWaves * 32 * 33 * 4, "the write-out fits the panels' memory");
-	__shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+	static_assert(STAGES * kStage >= kWaves * 32 * 33 * 4, "the write-out fits the panels' memory");
+	__shared__ __attribute__((aligned(1024))) char lds[STAGES * kStage];
 
 	const int lane = threadIdx.x & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	// consecutive groups go to different dies: give each die a run of neighbouring tiles
-	uint32_t t = blockIdx.x;
-	{
-		const uint32_t q = gridDim.x >> 3, rem = gridDim.x & 7, die = t & 7, at = t >> 3;
-		t = die * q + (die < rem ? die : rem) + at;
-	}
 	uint32_t tp, tq;
-	if (KIND == kNsGram || KIND == kNsPoly) {  // row tp of the lower triangle holds tp + 1 tiles
-		tp = (uint32_t)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
-		while (tp * (tp + 1) / 2 > t) tp--;
-		while ((tp + 1) * (tp + 2) / 2 <= t) tp++;
-		tq = t - tp * (tp + 1) / 2;
-	} else {
-		tp = t / g.tiles_q;
-		tq = t - tp * g.tiles_q;
-	}
+	tile_of_group<KIND>(g, tp, tq);
 	const size_t stride = (size_t)g.k_blocks * kNsBlock;
 	const char* P = g.P + blockIdx.y * g.batch_p + (size_t)tp * TP * stride;
 	const char* Q = g.Q + blockIdx.y * g.batch_q + (size_t)tq * TQ * stride;
@@ -196,30 +296,44 @@ __global__ __launch_bounds__(WP* WQ * 64) void ns_product_kernel(const NsArgs g)
 	}
 	const uint32_t lds0 = lds_offset(lds) + first_row * kNsBlock;
 
-	floatx16 acc[SP][SQ];
+	// With one 32 x 32 tile per wave every product would wait for the one before: four accumulators in turn.
+	constexpr int kChains = SP * SQ == 1 ? 4 : 1;
+	floatx16 acc[SP][SQ][kChains];
 #pragma unroll
 	for (int i = 0; i < SP; i++)
 #pragma unroll
 		for (int j = 0; j < SQ; j++)
 #pragma unroll
-			for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+			for (int c = 0; c < kChains; c++)
+#pragma unroll
+				for (int r = 0; r < 16; r++) acc[i][j][c][r] = 0.0f;
 
 	const int wp = wave / WQ, wq = wave % WQ;
 	const int swizzle = ((lane & 31) >> 1) & 7;
 	const char* frag_p = lds + (wp * SP * 32 + (lane & 31)) * kNsBlock;
 	const char* frag_q = lds + (TP + wq * SQ * 32 + (lane & 31)) * kNsBlock;
 
+	// A ring of STAGES stages: while one is multiplied, the next STAGES - 1 are on their way.
+	const uint32_t steps = g.k_blocks;
+	uint32_t fetched = 0, fill = 0;  // steps asked for; where the next one goes
+	auto fetch = [&]() {
 #pragma unroll
-	for (int i = 0; i < kLoads; i++) load_to_lds(lds0 + i * 1024, offset[i], src);
-	for (uint32_t k = 0; k < g.k_blocks; k++) {
-		asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-		__syncthreads();  // this step's panels are there, the other buffer has been read by everyone
-		const uint32_t cur = (k & 1) * kStage;
-		if (k + 1 < g.k_blocks) {
-			src += kNsBlock;
-#pragma unroll
-			for (int i = 0; i < kLoads; i++) load_to_lds(lds0 + (kStage - cur) + i * 1024, offset[i], src);
-		}
+		for (int i = 0; i < kLoads; i++) load_to_lds(lds0 + fill + i * 1024, offset[i], src);
+		src += kNsBlock;
+		fetched++;
+		fill = fill + kStage == STAGES * kStage ? 0 : fill + kStage;
+	};
+	for (int k = 0; k < STAGES - 1; k++)
+		if (fetched < steps) fetch();
+	uint32_t cur = 0;
+	for (uint32_t k = 0; k < steps; k++) {
+		// this step's panels are complete when at most the loads of the STAGES - 2 steps behind it are left
+		if (fetched - k == STAGES - 1)
+			wait_loads<(STAGES - 2) * kLoads>();
+		else
+			wait_loads<0>();
+		__syncthreads();  // everybody's part of the panels is there, and everybody has read the stage before
+		if (fetched < steps) fetch();
 #pragma unroll
 		for (int h = 0; h < 2; h++) {
 			const int hi_at = ((2 * h + (lane >> 5)) ^ swizzle) << 4, lo_at = hi_at ^ 64;
@@ -238,11 +352,14 @@ __global__ __launch_bounds__(WP* WQ * 64) void ns_product_kernel(const NsArgs g)
 			for (int i = 0; i < SP; i++)
 #pragma unroll
 				for (int j = 0; j < SQ; j++) {
-					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_lo[i], q_hi[j], acc[i][j], 0, 0, 0);
-					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi[i], q_lo[j], acc[i][j], 0, 0, 0);
-					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi[i], q_hi[j], acc[i][j], 0, 0, 0);
+					floatx16& low = acc[i][j][kChains == 1 ? 0 : h];
+					floatx16& high = acc[i][j][kChains == 1 ? 0 : 2 + h];
+					low = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_lo[i], q_hi[j], low, 0, 0, 0);
+					low = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi[i], q_lo[j], low, 0, 0, 0);
+					high = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi[i], q_hi[j], high, 0, 0, 0);
 				}
 		}
+		cur = cur + kStage == STAGES * kStage ? 0 : cur + kStage;
 	}
 	__syncthreads();  // the panels' memory becomes the waves' corners of the write-out
 
@@ -255,33 +372,100 @@ __global__ __launch_bounds__(WP* WQ * 64) void ns_product_kernel(const NsArgs g)
 			const uint32_t row0 = p0 + i * 32, col0 = q0 + j * 32;
 			float v[16];
 #pragma unroll
-			for (int r = 0; r < 16; r++) v[r] = g.alpha * acc[i][j][r];
-			if (KIND != kNsGram) {
-				// stored turned, so that the four rows of a lane are four neighbours
-				const char* a = g.addend + blockIdx.y * g.batch_addend + (size_t)(col0 + (lane & 31)) * g.addend_stride + (size_t)row0 * 4 + 8 * (lane >> 5);
-#pragma unroll
-				for (int q = 0; q < 4; q++) {
-					const half4 hi = *reinterpret_cast<const half4*>(a + 16 * q), lo = *reinterpret_cast<const half4*>(a + 16 * q + 64);
-#pragma unroll
-					for (int r = 0; r < 4; r++) v[4 * q + r] += g.beta * ((float)hi[r] + (float)lo[r]);
-				}
-			}
-			if (KIND == kNsLast) {
-				float* out = reinterpret_cast<float*>(reinterpret_cast<char*>(g.out) + blockIdx.y * g.batch_out);
-				const size_t col = col0 + (lane & 31);
-#pragma unroll
-				for (int r = 0; r < 16; r++) {
-					const size_t row = row0 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-					if (row < g.out_rows && col < g.out_cols) out[row * g.out_cols + col] = v[r];
-				}
-			} else {
-				char* straight = g.straight + blockIdx.y * g.batch_out + (size_t)row0 * g.straight_stride + (size_t)col0 * 4;
-				char* turned = g.turned + blockIdx.y * g.batch_out + (size_t)col0 * g.turned_stride + (size_t)row0 * 4;
-				// a tile on the diagonal is its own mirror: each of its elements has one writer
-				if ((KIND == kNsGram || KIND == kNsPoly) && tp == tq) turned = nullptr;
-				store_split_tile(v, corner, straight, g.straight_stride, turned, g.turned_stride);
-			}
+			for (int r = 0; r < 16; r++) v[r] = kChains == 1 ? acc[i][j][0][r] : (acc[i][j][0][r] + acc[i][j][kChains > 1][r]) + (acc[i][j][kChains / 2][r] + acc[i][j][kChains - 1][r]);
+			Addend a;
+			if (KIND != kNsGram) load_addend(g, a, row0, col0);
+			finish_tile<KIND>(g, v, a, row0, col0, tp == tq, corner);
 		}
+}
+
+// Few tiles: what counts is the way from the first load to the last store. A group of eight waves owns a 32 x 32 tile; each
+// wave multiplies the whole tile for 16 columns of every step of 128, and the waves' sums meet at the end. A wave fetches
+// the rows of one operand for one of a step's four blocks of columns; blocks beyond the end are skipped. (256 x 256, two
+// matrices: 5.3 us a product against 6.3 with 64 x 64 tiles and one wave per quarter; 64 x 64 tiles in this form: 7.4.)
+constexpr int kDeepWaves = 8, kDeepStages = 2;
+template <int KIND>
+__global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const NsArgs g) {
+	constexpr int T = 32, kBlocks = kDeepWaves / 2, kLoads = T / 8;
+	constexpr int kPanel = 2 * T * kNsBlock, kStage = kBlocks * kPanel;
+	static_assert(kDeepStages * kStage >= kDeepWaves * T * T * 4, "the waves' sums fit the panels' memory, and so does the write-out");
+	__shared__ __attribute__((aligned(1024))) char lds[kDeepStages * kStage];
+	const int lane = threadIdx.x & 63;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	uint32_t tp, tq;
+	tile_of_group<KIND>(g, tp, tq);
+	const size_t stride = (size_t)g.k_blocks * kNsBlock;
+	const uint32_t block = wave >> 1;
+	const char* src = (wave & 1 ? g.Q + blockIdx.y * g.batch_q + (size_t)tq * T * stride : g.P + blockIdx.y * g.batch_p + (size_t)tp * T * stride) + block * kNsBlock;
+	uint32_t offset[kLoads];
+#pragma unroll
+	for (int i = 0; i < kLoads; i++) {
+		const uint32_t row = i * 8 + (lane >> 3);
+		offset[i] = row * (uint32_t)stride + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+	}
+	const uint32_t lds0 = lds_offset(lds) + block * kPanel + (wave & 1) * T * kNsBlock;
+
+	const uint32_t steps = (g.k_blocks + kBlocks - 1) / kBlocks;
+	uint32_t fetched = 0, fill = 0;
+	auto fetch = [&]() {
+		if (fetched * kBlocks + block < g.k_blocks) {
+#pragma unroll
+			for (int i = 0; i < kLoads; i++) load_to_lds(lds0 + fill + i * 1024, offset[i], src);
+		}
+		src += kBlocks * kNsBlock;
+		fetched++;
+		fill = fill + kStage == kDeepStages * kStage ? 0 : fill + kStage;
+	};
+	fetch();
+	Addend addend;
+	if (KIND != kNsGram && wave == 0) load_addend(g, addend, tp * T, tq * T);  // arrives while the products run
+
+	floatx16 acc;
+#pragma unroll
+	for (int r = 0; r < 16; r++) acc[r] = 0.0f;
+	const int hi_at = ((2 * (wave & 1) + (lane >> 5)) ^ (((lane & 31) >> 1) & 7)) << 4, lo_at = hi_at ^ 64;
+	const char* frag_p = lds + block * kPanel + (lane & 31) * kNsBlock;
+	const char* frag_q = frag_p + T * kNsBlock;
+	uint32_t cur = 0;
+	for (uint32_t k = 0; k < steps; k++) {
+		wait_loads<0>();
+		__syncthreads();  // everybody's part of this step is there, and everybody has read the step before
+		if (fetched < steps) fetch();
+		if (k * kBlocks + block < g.k_blocks) {
+			const half8 p_hi = *reinterpret_cast<const half8*>(frag_p + cur + hi_at), p_lo = *reinterpret_cast<const half8*>(frag_p + cur + lo_at);
+			const half8 q_hi = *reinterpret_cast<const half8*>(frag_q + cur + hi_at), q_lo = *reinterpret_cast<const half8*>(frag_q + cur + lo_at);
+			acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_lo, q_hi, acc, 0, 0, 0);
+			acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi, q_lo, acc, 0, 0, 0);
+			acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi, q_hi, acc, 0, 0, 0);
+		}
+		cur = kStage - cur;
+	}
+	__syncthreads();
+
+	// the waves' sums: [wave][4 quarters][lane] of four floats
+	float4* sums = reinterpret_cast<float4*>(lds);
+#pragma unroll
+	for (int q = 0; q < 4; q++) sums[(wave * 4 + q) * 64 + lane] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+	__syncthreads();
+	if (wave != 0) return;
+	float v[16];
+#pragma unroll
+	for (int q = 0; q < 4; q++) {
+		float4 t = sums[q * 64 + lane];
+#pragma unroll
+		for (int w = 1; w < kDeepWaves; w++) {
+			const float4 u = sums[(w * 4 + q) * 64 + lane];
+			t.x += u.x;
+			t.y += u.y;
+			t.z += u.z;
+			t.w += u.w;
+		}
+		v[4 * q] = t.x;
+		v[4 * q + 1] = t.y;
+		v[4 * q + 2] = t.z;
+		v[4 * q + 3] = t.w;
+	}
+	finish_tile<KIND>(g, v, addend, tp * T, tq * T, tp == tq, reinterpret_cast<uint32_t*>(lds));
 }
 
 // ---- the host's side --------------------------------------------------------------------------------
@@ -322,26 +506,56 @@ static double scale_for(double bound) {
 	return ldexp(1.0, 15 - e);
 }
 
+// The tile of a product whose result is m x n (half of m x m for the symmetric kinds). A larger tile reads less per product
+// but leaves compute units idle. The measured time of a step of 32 columns over all of the result is close to a line in the
+// number n of tiles, in ns on 256 units: 130 + 0.5 n with tiles of 32, 220 + 1.1 n with 64, 500 + 2.7 n with 128, and
+// 3.3 n + 1900 for each round of the units with 256, of which only one fits a unit. The smallest wins. Measured, us per
+// product, smaller | larger tile:
+//   32 | 64:   X of 768 x 768 14.7 | 12.0, its A 9.2 | 11.7;      64 | 128: A of 2048 x 2048 45 | 54, its X 76.5 | 64.7
+//   128 | 256: X of 3000 x 3000 206 | 212, of 4096 x 4096 388 | 354; its A 251 | 262 (136 tiles of 256 on 256 units)
+static int ns_tile(size_t m, size_t n, bool half, size_t batch) {
+	static const int tiles[4] = {32, 64, 128, 256};
+	static const double base[4] = {130.0, 220.0, 500.0, 1900.0}, slope[4] = {0.5, 1.1, 2.7, 3.3};
+	int best = 0;
+	double least = 0.0;
+	for (int i = 0; i < 4; i++) {
+		const size_t tm = (m + tiles[i] - 1) / tiles[i], tn = (n + tiles[i] - 1) / tiles[i];
+		const double count = (double)batch * (half ? tm * (tm + 1) / 2 : tm * tn) * 256.0 / state().compute_units;
+		const double time = base[i] * (i == 3 ? ceil(count / 256.0) : 1.0) + slope[i] * count;
+		if (i == 0 || time < least) {
+			least = time;
+			best = tiles[i];
+		}
+	}
+	return best;
+}
+
 template <int KIND>
-static int ns_product(const NsArgs& a, int tile, size_t batch) {
-	const bool half = KIND == kNsGram || KIND == kNsPoly;
-	const unsigned tiles = half ? a.tiles_p * (a.tiles_p + 1) / 2 : a.tiles_p * a.tiles_q;
+static int ns_product(const NsArgs& args, int tile, size_t p_rows, size_t q_rows, size_t batch) {
+	NsArgs a = args;
+	a.tiles_p = (uint32_t)(p_rows / tile);
+	a.tiles_q = (uint32_t)(q_rows / tile);
+	const unsigned tiles = KIND == kNsGram || KIND == kNsPoly ? a.tiles_p * (a.tiles_p + 1) / 2 : a.tiles_p * a.tiles_q;
+	a.band = (uint32_t)sqrt(tiles / 8.0);
+	if (a.band < 1) a.band = 1;
 	const dim3 grid(tiles, (unsigned)batch);
-	if (tile == 128)
-		hipLaunchKernelGGL((ns_product_kernel<128, 128, 2, 2, KIND>), grid, dim3(256), 0, state().stream, a);
-	else
-		hipLaunchKernelGGL((ns_product_kernel<64, 64, 2, 2, KIND>), grid, dim3(256), 0, state().stream, a);
+	hipStream_t stream = state().stream;
+	switch (tile) {
+		case 32: hipLaunchKernelGGL(ns_product_deep_kernel<KIND>, grid, dim3(kDeepWaves * 64), 0, stream, a); break;
+		case 64: hipLaunchKernelGGL((ns_product_kernel<64, 64, 2, 2, 3, KIND>), grid, dim3(256), 0, stream, a); break;
+		case 128: hipLaunchKernelGGL((ns_product_kernel<128, 128, 2, 4, 2, KIND>), grid, dim3(512), 0, stream, a); break;
+		default: hipLaunchKernelGGL((ns_product_kernel<256, 256, 2, 4, 2, KIND>), grid, dim3(512), 0, stream, a); break;
+	}
 	TFHIP_CHECK_LAUNCH();
 	return TFHIP_OK;
 }
 
-static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps) {
+// `batch` matrices whose work space fits the arena together.
+static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps, int tile_half, int tile_full, size_t mp, size_t np) {
 	State& s = state();
 	const bool transposed = rows > cols;
 	const size_t m = transposed ? cols : rows, n = transposed ? rows : cols, elements = rows * cols;
-	const int tile = m > 512 ? 128 : 64;
-	const size_t mp = (m + tile - 1) / tile * tile, np = (n + tile - 1) / tile * tile;
-	const unsigned parts = (unsigned)(elements < 4096 ? 1 : elements / 4096 < 256 ? elements / 4096 : 256);
+	const unsigned parts = (unsigned)(elements < 4096 ? 1 : elements / 4096 < 512 ? elements / 4096 : 512);
 	auto align = [](size_t b) { return (b + 255) & ~size_t(255); };
 	const size_t norm_bytes = align(batch * parts * sizeof(double)), x_bytes = align(batch * mp * np * 4), a_bytes = align(batch * mp * mp * 4);
 	char* base = (char*)scratch(norm_bytes + 4 * x_bytes + 2 * a_bytes);
@@ -354,68 +568,67 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 	char* A = xt_next + x_bytes;
 	char* B = A + a_bytes;
 
-	hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)batch * parts), dim3(256), 0, s.stream, g, partial, elements, parts);
+	hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)batch * parts), dim3(256), 0, s.stream, g, partial, elements, parts, (elements & 3) == 0 && ((uintptr_t)g & 15) == 0);
 	TFHIP_CHECK_LAUNCH();
 	double bound = 1.0;
 	double scale_x = scale_for(bound);
-	hipLaunchKernelGGL(ns_split_kernel, dim3((unsigned)((mp / 32 * (np / 32) + 3) / 4), (unsigned)batch), dim3(256), 0, s.stream, g, (const double*)partial, parts, x, xt, m, n, mp, np, transposed, eps,
+	const size_t split_groups = (mp / 32 * (np / 32) + 3) / 4, most = (size_t)s.compute_units * 8;
+	hipLaunchKernelGGL(ns_split_kernel, dim3((unsigned)(split_groups < most ? split_groups : most), (unsigned)batch), dim3(256), 0, s.stream, g, (const double*)partial, parts, x, xt, m, n, mp, np, transposed, eps,
 	                   (float)scale_x);
 	TFHIP_CHECK_LAUNCH();
 	for (int k = 0; k < steps; k++) {
 		const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
-		// a bound that rounding does not cross
+		// bounds that rounding does not cross
 		const double scale_a = scale_for(bound * bound * 1.0001), scale_b = scale_for(largest_square(b, c, bound * bound) * 1.0001);
 		const double next = largest_quintic(a, b, c, bound) * 1.0001, scale_next = scale_for(next);
-		NsArgs args = {};
-		args.P = args.Q = x;
-		args.straight = args.turned = A;
-		args.straight_stride = args.turned_stride = mp * 4;
-		args.batch_p = args.batch_q = mp * np * 4;
-		args.batch_out = mp * mp * 4;
-		args.k_blocks = (uint32_t)(np / kNsStep);
-		args.tiles_p = args.tiles_q = (uint32_t)(mp / tile);
-		args.alpha = (float)(scale_a / (scale_x * scale_x));
-		int rc = ns_product<kNsGram>(args, tile, batch);
+		NsArgs gram = {};
+		gram.P = gram.Q = x;
+		gram.straight = gram.turned = A;
+		gram.straight_stride = gram.turned_stride = mp * 4;
+		gram.batch_p = gram.batch_q = mp * np * 4;
+		gram.batch_out = mp * mp * 4;
+		gram.k_blocks = (uint32_t)(np / kNsStep);
+		gram.alpha = (float)(scale_a / (scale_x * scale_x));
+		int rc = ns_product<kNsGram>(gram, tile_half, mp, mp, batch);
 		if (rc) return rc;
-		args.P = args.Q = A;
-		args.straight = args.turned = B;
-		args.batch_p = args.batch_q = mp * mp * 4;
-		args.k_blocks = (uint32_t)(mp / kNsStep);
-		args.alpha = (float)(c * scale_b / (scale_a * scale_a));
-		args.beta = (float)(b * scale_b / scale_a);
-		args.addend = A;
-		args.addend_stride = mp * 4;
-		args.batch_addend = mp * mp * 4;
-		rc = ns_product<kNsPoly>(args, tile, batch);
+		NsArgs poly = gram;
+		poly.P = poly.Q = poly.addend = A;
+		poly.straight = poly.turned = B;
+		poly.batch_p = poly.batch_q = poly.batch_addend = mp * mp * 4;
+		poly.addend_stride = mp * 4;
+		poly.k_blocks = (uint32_t)(mp / kNsStep);
+		poly.alpha = (float)(c * scale_b / (scale_a * scale_a));
+		poly.beta = (float)(b * scale_b / scale_a);
+		rc = ns_product<kNsPoly>(poly, tile_half, mp, mp, batch);
 		if (rc) return rc;
 		const bool last = k + 1 == steps;
 		const bool turn = last && transposed;  // the caller's rows are the columns of X
-		args.P = turn ? xt : B;
-		args.Q = turn ? B : xt;
-		args.batch_p = turn ? mp * np * 4 : mp * mp * 4;
-		args.batch_q = turn ? mp * mp * 4 : mp * np * 4;
-		args.addend = turn ? x : xt;
-		args.addend_stride = (turn ? np : mp) * 4;
-		args.batch_addend = mp * np * 4;
-		args.tiles_p = (uint32_t)((turn ? np : mp) / tile);
-		args.tiles_q = (uint32_t)((turn ? mp : np) / tile);
+		NsArgs update = {};
+		update.P = turn ? xt : B;
+		update.Q = turn ? B : xt;
+		update.batch_p = turn ? mp * np * 4 : mp * mp * 4;
+		update.batch_q = turn ? mp * mp * 4 : mp * np * 4;
+		update.addend = turn ? x : xt;
+		update.addend_stride = (turn ? np : mp) * 4;
+		update.batch_addend = mp * np * 4;
+		update.k_blocks = (uint32_t)(mp / kNsStep);
 		if (last) {
-			args.out = out;
-			args.out_rows = rows;
-			args.out_cols = cols;
-			args.batch_out = elements * sizeof(float);
-			args.alpha = (float)(1.0 / (scale_b * scale_x));
-			args.beta = (float)(a / scale_x);
-			rc = ns_product<kNsLast>(args, tile, batch);
+			update.out = out;
+			update.out_rows = rows;
+			update.out_cols = cols;
+			update.batch_out = elements * sizeof(float);
+			update.alpha = (float)(1.0 / (scale_b * scale_x));
+			update.beta = (float)(a / scale_x);
+			rc = ns_product<kNsLast>(update, tile_full, turn ? np : mp, turn ? mp : np, batch);
 		} else {
-			args.straight = x_next;
-			args.turned = xt_next;
-			args.straight_stride = np * 4;
-			args.turned_stride = mp * 4;
-			args.batch_out = mp * np * 4;
-			args.alpha = (float)(scale_next / (scale_b * scale_x));
-			args.beta = (float)(a * scale_next / scale_x);
-			rc = ns_product<kNsUpdate>(args, tile, batch);
+			update.straight = x_next;
+			update.turned = xt_next;
+			update.straight_stride = np * 4;
+			update.turned_stride = mp * 4;
+			update.batch_out = mp * np * 4;
+			update.alpha = (float)(scale_next / (scale_b * scale_x));
+			update.beta = (float)(a * scale_next / scale_x);
+			rc = ns_product<kNsUpdate>(update, tile_full, mp, np, batch);
 		}
 		if (rc) return rc;
 		char* t = x;
@@ -450,5 +663,18 @@ extern "C" int tfhip_newton_schulz_f32(const float* g, float* out, size_t batch,
 	if (g != out && words_overlap(g, batch * rows * cols, out, batch * rows * cols)) return fail(TFHIP_ERR_ARG, "Newton-Schulz: g and out overlap without being the same");
 	TFHIP_REQUIRE_INIT();
 	TFHIP_HOLD_DEVICE();
-	return newton_schulz(g, out, batch, rows, cols, steps, coefficients, eps);
+	// As many matrices at a time as a work space of 4 GiB holds, at least one.
+	const size_t at_once = batch < 256 ? batch : 256;
+	const int tile_half = ns_tile(shorter, shorter, true, at_once), tile_full = ns_tile(shorter, longer, false, at_once);
+	const size_t tile = tile_half > tile_full ? tile_half : tile_full;
+	const size_t mp = (shorter + tile - 1) / tile * tile, np = (longer + tile - 1) / tile * tile;
+	size_t chunk = ((size_t)4 << 30) / (16 * mp * np + 8 * mp * mp);
+	if (chunk < 1) chunk = 1;
+	if (chunk > batch) chunk = batch;
+	for (size_t first = 0; first < batch; first += chunk) {
+		const size_t count = batch - first < chunk ? batch - first : chunk;
+		const int rc = newton_schulz(g + first * rows * cols, out + first * rows * cols, count, rows, cols, steps, coefficients, eps, tile_half, tile_full, mp, np);
+		if (rc) return rc;
+	}
+	return TFHIP_OK;
 }

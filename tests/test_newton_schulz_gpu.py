@@ -164,3 +164,18 @@ def test_word_aligned_addresses(rt):
     whole.write(g.reshape(-1), offset_words=1)
     rt.newton_schulz(rt.DeviceBuffer.view(whole.ptr + 4, g.size), rt.DeviceBuffer.view(out.ptr + 12, g.size), 70, 90)
     assert np.array_equal(out.numpy(np.float32, g.shape, offset_words=3), run(rt, g))
+
+
+@pytest.mark.parametrize("batch, shape", [(4, (1000, 1020)), (16, (1020, 1000)), (16, (1000, 1020)), (25, (1000, 1020)), (1, (2100, 2051)), (1, (3600, 65))])
+def test_many_tiles(rt, batch, shape):
+    """Enough work for the large tiles (128 and 256 rows and columns), with ragged edges, against float64 for the first and the
+    last matrix of the batch; and the same words when it runs again."""
+    rng = np.random.default_rng([batch, *shape])
+    g = (rng.standard_normal((batch, *shape), dtype=np.float32) + rng.standard_normal((batch, shape[0], 4), dtype=np.float32) @ rng.standard_normal((batch, 4, shape[1]), dtype=np.float32))
+    steps = 2
+    got = run(rt, g, batch=batch, steps=steps)
+    for k in {0, batch - 1}:
+        want = newton_schulz64(g[k], steps)
+        # two steps: the first's error grows by at most 3.4445
+        assert np.linalg.norm(got[k] - want) <= 3 * 3.5 * e(max(shape)) * np.linalg.norm(want)
+    assert np.array_equal(run(rt, g, batch=batch, steps=steps), got)
