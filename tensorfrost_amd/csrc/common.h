@@ -62,6 +62,8 @@ int check_async_error();
 
 // What tfhip_radix_sort_kv takes of the scratch arena, from its front, for n keys whose ping-pong buffers the caller gives.
 size_t radix_sort_scratch_bytes(size_t n);
+// tfhip_radix_sort_kv_u32 of keys below 256^digits (1 to 4), all six buffers given: one pass per digit.
+int radix_sort_low_digits(const uint32_t* keys_in, const uint32_t* vals_in, uint32_t* keys_out, uint32_t* vals_out, uint32_t* keys_tmp, uint32_t* vals_tmp, size_t n, int digits);
 
 // Finds the device address of the fixed status-word array of the allocation-free scan on `device`, which must be the
 // current device (every GPU holds its own copy at its own address). Called by tfhip_init.

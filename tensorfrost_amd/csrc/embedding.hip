@@ -76,98 +76,157 @@ __global__ __launch_bounds__(256) void embedding_kernel(const int32_t* __restric
 
 // ---- the order of the positions ----------------------------------------------------------------------
 
-// A position's key is its token, or vocab where the token names no row. The sorted keys and positions of a tile come
-// from counting: the place of position i is the number of keys that are smaller, or equal and earlier. A group places 64
-// positions; its four waves each compare them with a quarter of the tile's keys, a compare and an add per pair:
-// tile * 64 pairs take about 2 tile cycles. Up to kAllPairs positions are one tile; beyond, tiles of kSortTile are sorted
-// so and merged by searches.
-constexpr uint32_t kAllPairs = 8192, kSortTile = 1024, kMostSearched = 131072;
-
-__device__ __forceinline__ uint32_t token_key(int32_t t, uint32_t vocab) { return t >= 0 && (uint32_t)t < vocab ? (uint32_t)t : vocab; }
-
-__global__ __launch_bounds__(256) void embedding_count_kernel(const int32_t* __restrict__ tokens, uint32_t* __restrict__ keys, uint32_t* __restrict__ order, uint32_t n, uint32_t vocab,
-                                                              uint32_t tile) {
-	__shared__ __attribute__((aligned(16))) uint32_t key[kAllPairs];
-	__shared__ uint32_t counts[4][64];
-	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-	const uint32_t first = blockIdx.x * 64 / tile * tile;              // the tile's first position
-	const uint32_t count = n - first < tile ? n - first : tile;
-	const uint32_t blocks = (count + 63) / 64;
-	for (uint32_t i = threadIdx.x; i < blocks * 64; i += 256) key[i] = i < count ? token_key(tokens[first + i], vocab) : 0xFFFFFFFFu;
-	__syncthreads();
-	const uint32_t mine = blockIdx.x * 64 - first + lane, my_block = mine / 64;
-	const uint32_t k = key[mine];
+// Up to kAllPairs positions by counting: the place of position i is the number of keys that are smaller, or equal and
+// earlier. A key is the token read as unsigned: what names no row (negative, or beyond the table) is at least vocab and comes
+// last. A group places 64 positions, one per lane of each of its waves; the waves each compare them with their share of
+// the keys: a lane broadcast, a compare and an add per pair. 500 positions 4.7 us, 4096 9, 8192 16 (the kernels below 16).
+constexpr uint32_t kAllPairs = 4096;
+constexpr int kCountWaves = 16;
+__global__ __launch_bounds__(kCountWaves * 64) void embedding_count_kernel(const uint32_t* __restrict__ tokens, uint32_t* __restrict__ keys, uint32_t* __restrict__ order, uint32_t n) {
+	__shared__ uint32_t counts[kCountWaves][64];
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const uint32_t my_block = blockIdx.x, mine = my_block * 64 + lane;
+	const uint32_t k = mine < n ? tokens[mine] : 0;
 	uint32_t before = 0;
-	for (uint32_t b = wave; b < blocks; b += 4) {
-		const uint4* other = reinterpret_cast<const uint4*>(key + b * 64);
-		if (b != my_block) {
-			const uint32_t below = b < my_block ? k + 1 : k;  // equal keys count when they stand before
+	for (uint32_t b0 = wave; b0 * 64 < n; b0 += 4 * kCountWaves) {
+		uint32_t other[4];  // four blocks of 64 keys, one key per lane
 #pragma unroll
-			for (int j = 0; j < 16; j++) {
-				const uint4 o = other[j];
-				before += (o.x < below) + (o.y < below) + (o.z < below) + (o.w < below);
+		for (int u = 0; u < 4; u++) {
+			const uint32_t at = (b0 + u * kCountWaves) * 64 + lane;
+			other[u] = at < n ? tokens[at] : 0xFFFFFFFFu;  // smaller than nothing, and behind every position
+		}
+#pragma unroll
+		for (int u = 0; u < 4; u++) {
+			const uint32_t b = b0 + u * kCountWaves;
+			if (b * 64 >= n) break;
+			if (b < my_block) {  // equal keys count: they stand before
+#pragma unroll
+				for (int j = 0; j < 64; j++) before += (uint32_t)__builtin_amdgcn_readlane(other[u], j) <= k;
+			} else {
+#pragma unroll
+				for (int j = 0; j < 64; j++) before += (uint32_t)__builtin_amdgcn_readlane(other[u], j) < k;
+				if (b == my_block) {
+#pragma unroll
+					for (int j = 0; j < 64; j++) before += (uint32_t)__builtin_amdgcn_readlane(other[u], j) == k && j < lane;
+				}
 			}
-		} else {
-			for (int j = 0; j < 64; j++) before += key[b * 64 + j] < k + (j < lane);
 		}
 	}
 	counts[wave][lane] = before;
 	__syncthreads();
-	if (wave == 0 && mine < count) {
-		const uint32_t at = first + counts[0][lane] + counts[1][lane] + counts[2][lane] + counts[3][lane];
+	if (wave == 0 && mine < n) {
+		uint32_t at = 0;
+#pragma unroll
+		for (int w = 0; w < kCountWaves; w++) at += counts[w][lane];
 		keys[at] = k;
-		order[at] = first + mine;
+		order[at] = mine;
 	}
 }
 
-// Merges sorted tiles of kSortTile: the place of an element is its place in its own tile plus, for every other tile, the
-// number of that tile's keys that come before it (binary search in group memory; tiles before count equal keys, tiles
-// behind do not). A group places 256 elements; four threads share an element and search a tile each of the four
-// that a thread group has in flight. The last tile may be short: it is filled up with the largest key.
-constexpr int kMergeTiles = 16;
-__global__ __launch_bounds__(1024) void embedding_merge_kernel(const uint32_t* __restrict__ tile_keys, const uint32_t* __restrict__ tile_order, uint32_t* __restrict__ keys,
-                                                               uint32_t* __restrict__ order, uint32_t n) {
-	__shared__ uint32_t lds[kMergeTiles * kSortTile];
-	__shared__ uint32_t counts[4][256];
-	const uint32_t item = threadIdx.x & 255, quarter = threadIdx.x >> 8;
-	const uint32_t e = blockIdx.x * 256 + item, tile = blockIdx.x * 256 / kSortTile, tiles = (n + kSortTile - 1) / kSortTile;
-	const uint32_t k = e < n ? tile_keys[e] : 0xFFFFFFFEu;
-	uint32_t before = 0;
-	for (uint32_t t0 = 0; t0 < tiles; t0 += kMergeTiles) {
-		__syncthreads();
-#pragma unroll
-		for (int i = 0; i < kMergeTiles; i++) {
-			const uint32_t at = (t0 + i) * kSortTile + threadIdx.x;
-			lds[i * kSortTile + threadIdx.x] = at < n ? tile_keys[at] : 0xFFFFFFFFu;
-		}
-		__syncthreads();
-		uint32_t found[4] = {0, 0, 0, 0}, below[4];
-#pragma unroll
-		for (int i = 0; i < 4; i++) below[i] = t0 + quarter * 4 + i < tile ? k + 1 : k;
-#pragma unroll
-		for (uint32_t half = kSortTile / 2; half >= 1; half /= 2)
-#pragma unroll
-			for (int i = 0; i < 4; i++) found[i] += lds[(quarter * 4 + i) * kSortTile + found[i] + half - 1] < below[i] ? half : 0;
-#pragma unroll
-		for (int i = 0; i < 4; i++) {
-			found[i] += lds[(quarter * 4 + i) * kSortTile + found[i]] < below[i];  // found <= kSortTile - 1 here
-			if (t0 + quarter * 4 + i != tile) before += found[i];
-		}
-	}
-	counts[quarter][item] = before;
+// Up to kMostTiled positions by a stable sort on 8-bit digits, as many as the table's size has, in tiles of kDigitTile
+// small enough that a few tens of thousands of positions spread over the chip (the library's sort, with its tiles of 16384,
+// takes 14 us a pass whatever little it is given, and clears and scans its counters in launches of their own). Counts are
+// kept per tile and digit; a group finds where its keys of a digit go by adding up all tiles' counts itself. (Counting the
+// next digit while this pass's keys are written, by atomics, saves a launch of 4.8 us and costs 13: the frequent tokens meet on
+// a few counters.)
+constexpr uint32_t kDigitTile = 1024, kMostTiled = 131072;
+
+__device__ __forceinline__ uint32_t known_key(int32_t t, uint32_t vocab) { return t >= 0 && (uint32_t)t < vocab ? (uint32_t)t : vocab; }
+
+// counts[tile][256] of one digit; FIRST reads the tokens.
+template <bool FIRST>
+__global__ __launch_bounds__(256) void embedding_digits_kernel(const int32_t* __restrict__ tokens, const uint32_t* __restrict__ keys, uint32_t* __restrict__ counts, uint32_t n, uint32_t vocab,
+                                                               int shift) {
+	__shared__ uint32_t count[256];
+	count[threadIdx.x] = 0;
 	__syncthreads();
-	if (quarter == 0 && e < n) {
-		const uint32_t at = e - tile * kSortTile + counts[0][item] + counts[1][item] + counts[2][item] + counts[3][item];
-		keys[at] = k;
-		order[at] = tile_order[e];
+#pragma unroll
+	for (int j = 0; j < 4; j++) {
+		const uint32_t i = blockIdx.x * kDigitTile + j * 256 + threadIdx.x;
+		if (i < n) atomicAdd(&count[((FIRST ? known_key(tokens[i], vocab) : keys[i]) >> shift) & 255u], 1u);
+	}
+	__syncthreads();
+	counts[blockIdx.x * 256 + threadIdx.x] = count[threadIdx.x];
+}
+
+// One pass: keys and positions to their places by digit `shift / 8`; FIRST reads the tokens.
+template <bool FIRST>
+__global__ __launch_bounds__(256) void embedding_scatter_kernel(const int32_t* __restrict__ tokens, const uint32_t* __restrict__ keys_in, const uint32_t* __restrict__ order_in,
+                                                                uint32_t* __restrict__ keys_out, uint32_t* __restrict__ order_out, const uint32_t* __restrict__ counts, uint32_t n,
+                                                                uint32_t vocab, uint32_t tiles, int shift) {
+	__shared__ uint32_t wave_count[4][256];
+	__shared__ uint32_t place[256];
+	__shared__ uint32_t wave_total[4];
+	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+	// wave w owns positions [256 w, 256 w + 256) of the tile; item j of lane l is number 64 j + l of them
+	const uint32_t base = blockIdx.x * kDigitTile + wave * 256 + lane;
+	uint32_t key[4], from[4];
+#pragma unroll
+	for (int j = 0; j < 4; j++) {
+		const uint32_t i = base + j * 64;
+		key[j] = i < n ? (FIRST ? known_key(tokens[i], vocab) : keys_in[i]) : 0xFFFFFFFFu;
+		from[j] = FIRST ? i : i < n ? order_in[i] : 0u;
+	}
+#pragma unroll
+	for (int w = 0; w < 4; w++) wave_count[w][tid] = 0;
+	// keys of digit `tid` in the tiles before this one, and in all
+	uint32_t before = 0, total = 0;
+	for (uint32_t t0 = 0; t0 < tiles; t0 += 8) {
+		uint32_t c[8];
+#pragma unroll
+		for (int u = 0; u < 8; u++) c[u] = t0 + u < tiles ? counts[(t0 + u) * 256 + tid] : 0u;
+#pragma unroll
+		for (int u = 0; u < 8; u++) {
+			total += c[u];
+			before += t0 + u < blockIdx.x ? c[u] : 0u;
+		}
+	}
+	uint32_t upto = total;
+#pragma unroll
+	for (int off = 1; off < 64; off <<= 1) {
+		const uint32_t o = __shfl_up(upto, off, 64);
+		if (lane >= off) upto += o;
+	}
+	if (lane == 63) wave_total[wave] = upto;
+	__syncthreads();
+	for (int w = 0; w < wave; w++) upto += wave_total[w];
+	place[tid] = upto - total + before;
+	// the rank of a key among those of its digit in its wave, in the order of the positions
+	uint32_t rank[4];
+#pragma unroll
+	for (int j = 0; j < 4; j++) {
+		const uint32_t d = (key[j] >> shift) & 255u;
+		uint64_t peers = __ballot(base + j * 64 < n);
+#pragma unroll
+		for (int b = 0; b < 8; b++) {
+			const bool bit = (d >> b) & 1u;
+			const uint64_t votes = __ballot(bit);
+			peers &= bit ? votes : ~votes;
+		}
+		const uint32_t ahead = __popcll(peers & ((1ull << lane) - 1));
+		const uint32_t seen = wave_count[wave][d];  // read by all peers before the last of them raises it
+		__builtin_amdgcn_wave_barrier();
+		if (base + j * 64 < n && ahead + 1 == (uint32_t)__popcll(peers)) wave_count[wave][d] = seen + ahead + 1;
+		__builtin_amdgcn_wave_barrier();
+		rank[j] = seen + ahead;
+	}
+	__syncthreads();
+#pragma unroll
+	for (int j = 0; j < 4; j++) {
+		if (base + j * 64 >= n) continue;
+		const uint32_t d = (key[j] >> shift) & 255u;
+		uint32_t at = place[d] + rank[j];
+		for (int w = 0; w < wave; w++) at += wave_count[w][d];
+		keys_out[at] = key[j];
+		order_out[at] = from[j];
 	}
 }
 
-// For the radix sort: keys[i] as above, order[i] = i.
+// For the library's sort, which takes more positions: keys[i] as above, order[i] = i.
 __global__ __launch_bounds__(256) void embedding_keys_kernel(const int32_t* __restrict__ tokens, uint32_t* __restrict__ keys, uint32_t* __restrict__ order, uint32_t n, uint32_t vocab) {
 	const uint32_t i = blockIdx.x * 256 + threadIdx.x;
 	if (i >= n) return;
-	keys[i] = token_key(tokens[i], vocab);
+	keys[i] = known_key(tokens[i], vocab);
 	order[i] = i;
 }
 
@@ -191,7 +250,7 @@ __device__ __forceinline__ uint32_t first_at_least(const uint32_t* __restrict__ 
 // [segment][0] what continues from the segment before (or fills the segment), [segment][1] what begins here and goes on.
 // The groups behind those of the segments write zeros into the rows that no position names, kZeroRows rows a wave:
 // whether a row is named is found by a search for it, all rows of a wave at once.
-constexpr int kSumRows = 8, kZeroRows = 16;
+constexpr int kSumRows = 8, kZeroRows = 8;
 
 template <int VEC>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ order, const float* __restrict__ dy, float* __restrict__ dtable,
@@ -209,18 +268,24 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const uint32_t* __re
 		if (key >= vocab) return;  // positions without a row come last
 		bool open = begin > 0 && keys[begin - 1] == key;  // the run began in an earlier segment
 		Vec sum = Vec(0.0f);
-		for (uint32_t p0 = begin; p0 < end; p0 += kSumRows) {
-			uint32_t k[kSumRows];
-			size_t row[kSumRows];
-			Vec v[kSumRows];
+		uint32_t k[kSumRows], next_k[kSumRows], next_row[kSumRows];
+		auto look_up = [&](uint32_t p0) {
 #pragma unroll
 			for (int u = 0; u < kSumRows; u++) {
 				const uint32_t p = p0 + u < end ? p0 + u : end - 1;
-				k[u] = keys[p];
-				row[u] = (size_t)order[p] * cols;
+				next_k[u] = keys[p];
+				next_row[u] = order[p];
 			}
+		};
+		look_up(begin);
+		for (uint32_t p0 = begin; p0 < end; p0 += kSumRows) {
+			Vec v[kSumRows];
 #pragma unroll
-			for (int u = 0; u < kSumRows; u++) v[u] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(dy + row[u] + c));
+			for (int u = 0; u < kSumRows; u++) {
+				k[u] = next_k[u];
+				v[u] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(dy + (size_t)next_row[u] * cols + c));
+			}
+			if (p0 + kSumRows < end) look_up(p0 + kSumRows);  // on its way while these rows arrive
 #pragma unroll
 			for (int u = 0; u < kSumRows; u++) {
 				if (p0 + u >= end) break;
@@ -288,7 +353,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embedding_join_kernel(const u
 		parts += __builtin_ctzll(~inside);
 		break;
 	}
-	for (size_t c0 = 0; c0 < cols; c0 += 64 * VEC) {
+	for (size_t c0 = (size_t)blockIdx.y * 64 * VEC; c0 < cols; c0 += (size_t)gridDim.y * 64 * VEC) {
 		const size_t c = c0 + (size_t)lane * VEC;
 		Vec sum = Vec(0.0f);
 		if (c < cols) {
@@ -326,7 +391,8 @@ static int embedding_sums(const uint32_t* keys, const uint32_t* order, const flo
 	                   lanes, (uint32_t)col_steps, (uint32_t)sum_groups);
 	TFHIP_CHECK_LAUNCH();
 	if (segments > 1) {
-		hipLaunchKernelGGL(embedding_join_kernel<VEC>, dim3(segments - 1), dim3(kJoinWaves * 64), 0, s.stream, keys, dtable, (const float*)partial, n, vocab, cols, scale, segment, segments);
+		const size_t stretches = (cols + 64 * VEC - 1) / (64 * VEC);
+		hipLaunchKernelGGL(embedding_join_kernel<VEC>, dim3(segments - 1, (unsigned)(stretches < 16 ? stretches : 16)), dim3(kJoinWaves * 64), 0, s.stream, keys, dtable, (const float*)partial, n, vocab, cols, scale, segment, segments);
 		TFHIP_CHECK_LAUNCH();
 	}
 	return TFHIP_OK;
@@ -376,30 +442,50 @@ extern "C" int tfhip_embedding_rows_backward_f32(const int32_t* tokens, const fl
 	TFHIP_HOLD_DEVICE();
 	State& s = state();
 	if (n == 0) return tfhip_fill_u32(dtable, 0u, vocab * cols);
-	const bool radix = n > kMostSearched;
-	const uint32_t segment = n * cols >= (size_t)1 << 22 ? 64 : 16;  // few rows: shorter chains of loads, more of them at once
+	const bool radix = n > kMostTiled;
+	int digits = 1;  // of keys 0 .. vocab
+	while (digits < 4 && vocab >> (8 * digits)) digits++;
+	// Rows a wave adds up one after the other: few rows need shorter chains, more of them at once (500 x 250: sums and
+	// joins 9.6 us with 16, 11.3 with 32, 16.5 with 64), many rows fewer parts to join (65536 x 1024: 93, 89 and 88.5 us).
+	const uint32_t segment = n * cols >= (size_t)1 << 22 ? 32 : 16;
 	const size_t segments = (n + segment - 1) / segment;
-	// [the sort's own words][keys, order sorted][keys, order before (and between) the sort's passes][parts of the runs]
+	// [the library sort's own words][keys, order sorted][keys, order between passes, and before them][counts][parts of the runs]
 	const size_t words = (n + 63) & ~size_t(63);
+	const uint32_t tiles = (uint32_t)((n + kDigitTile - 1) / kDigitTile);
 	const size_t sort_bytes = radix ? radix_sort_scratch_bytes(n) : 0, arrays = n <= kAllPairs ? 2 : radix ? 6 : 4;
-	char* base = (char*)scratch(sort_bytes + arrays * words * sizeof(uint32_t) + segments * 2 * cols * sizeof(float));
+	const size_t count_words = radix || n <= kAllPairs ? 0 : (size_t)tiles * 256;
+	char* base = (char*)scratch(sort_bytes + (arrays * words + count_words) * sizeof(uint32_t) + segments * 2 * cols * sizeof(float));
 	if (!base) return TFHIP_ERR_HIP;
 	uint32_t* keys = (uint32_t*)(base + sort_bytes);
 	uint32_t* order = keys + words;
-	float* partial = (float*)(keys + arrays * words);
+	uint32_t* counts = keys + arrays * words;
+	float* partial = (float*)(counts + count_words);
 	if (radix) {
 		hipLaunchKernelGGL(embedding_keys_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s.stream, tokens, keys + 2 * words, keys + 3 * words, (uint32_t)n, (uint32_t)vocab);
 		TFHIP_CHECK_LAUNCH();
-		rc = tfhip_radix_sort_kv_u32(keys + 2 * words, keys + 3 * words, keys, order, keys + 4 * words, keys + 5 * words, n);
+		rc = radix_sort_low_digits(keys + 2 * words, keys + 3 * words, keys, order, keys + 4 * words, keys + 5 * words, n, digits);
 		if (rc) return rc;
 	} else if (n > kAllPairs) {
-		hipLaunchKernelGGL(embedding_count_kernel, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, s.stream, tokens, keys + 2 * words, keys + 3 * words, (uint32_t)n, (uint32_t)vocab, kSortTile);
-		TFHIP_CHECK_LAUNCH();
-		hipLaunchKernelGGL(embedding_merge_kernel, dim3((unsigned)((n + 255) / 256)), dim3(1024), 0, s.stream, (const uint32_t*)(keys + 2 * words), (const uint32_t*)(keys + 3 * words), keys, order,
-		                   (uint32_t)n);
-		TFHIP_CHECK_LAUNCH();
+		for (int p = 0; p < digits; p++) {
+			// the last pass ends in keys and order
+			const bool away = (digits - 1 - p) & 1;
+			const uint32_t* from = away ? keys : keys + 2 * words;
+			uint32_t* to = away ? keys + 2 * words : keys;
+			const dim3 grid(tiles), block(256);
+			if (p == 0) {
+				hipLaunchKernelGGL(embedding_digits_kernel<true>, grid, block, 0, s.stream, tokens, from, counts, (uint32_t)n, (uint32_t)vocab, 0);
+				TFHIP_CHECK_LAUNCH();
+				hipLaunchKernelGGL(embedding_scatter_kernel<true>, grid, block, 0, s.stream, tokens, from, from + words, to, to + words, (const uint32_t*)counts, (uint32_t)n, (uint32_t)vocab, tiles, 0);
+			} else {
+				hipLaunchKernelGGL(embedding_digits_kernel<false>, grid, block, 0, s.stream, tokens, from, counts, (uint32_t)n, (uint32_t)vocab, 8 * p);
+				TFHIP_CHECK_LAUNCH();
+				hipLaunchKernelGGL(embedding_scatter_kernel<false>, grid, block, 0, s.stream, tokens, from, from + words, to, to + words, (const uint32_t*)counts, (uint32_t)n, (uint32_t)vocab, tiles,
+				                   8 * p);
+			}
+			TFHIP_CHECK_LAUNCH();
+		}
 	} else {
-		hipLaunchKernelGGL(embedding_count_kernel, dim3((unsigned)((n + 63) / 64)), dim3(256), 0, s.stream, tokens, keys, order, (uint32_t)n, (uint32_t)vocab, kAllPairs);
+		hipLaunchKernelGGL(embedding_count_kernel, dim3((unsigned)((n + 63) / 64)), dim3(kCountWaves * 64), 0, s.stream, (const uint32_t*)tokens, keys, order, (uint32_t)n);
 		TFHIP_CHECK_LAUNCH();
 	}
 	const RowShape r = row_shape(cols, dy, dtable);

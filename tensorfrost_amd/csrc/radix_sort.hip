@@ -364,7 +364,7 @@ size_t radix_sort_scratch_bytes(size_t n) {
 }
 
 static int radix_sort_impl(int kind, const uint32_t* keys_in, const uint32_t* vals_in, uint32_t* keys_out, uint32_t* vals_out,
-                           uint32_t* keys_tmp, uint32_t* vals_tmp, size_t n) {
+                           uint32_t* keys_tmp, uint32_t* vals_tmp, size_t n, int passes = 4) {
 	State& st = state();
 	// keys_out keeps the order-preserving unsigned form of the keys (what sort.py's own passes work on) when asked to
 	const bool keep_mapped = (kind & TFHIP_KEY_KEEP_MAPPED) != 0;
@@ -419,14 +419,15 @@ static int radix_sort_impl(int kind, const uint32_t* keys_in, const uint32_t* va
 	hipLaunchKernelGGL(radix_offsets_kernel, dim3(1), dim3(kRadix), 0, st.stream, (const uint32_t*)hist, offsets);
 	TFHIP_CHECK_LAUNCH();
 
-	// in -> tmp -> out -> tmp -> out
+	// in -> tmp -> out -> tmp -> out; fewer passes start so that the last one ends in out
 	const uint32_t* src_k = keys_in;
 	const uint32_t* src_v = vals_in;
-	for (int pass = 0; pass < 4; pass++) {
-		uint32_t* dst_k = (pass & 1) ? keys_out : keys_tmp;
-		uint32_t* dst_v = (pass & 1) ? vals_out : vals_tmp;
+	for (int pass = 0; pass < passes; pass++) {
+		const bool to_tmp = (passes - 1 - pass) & 1;
+		uint32_t* dst_k = to_tmp ? keys_tmp : keys_out;
+		uint32_t* dst_v = to_tmp ? vals_tmp : vals_out;
 		const bool enc = pass == 0 && kind != kKeyU32;
-		const bool dec = pass == 3 && kind != kKeyU32 && !keep_mapped;
+		const bool dec = pass == passes - 1 && kind != kKeyU32 && !keep_mapped;
 		if (has_vals)
 			hipLaunchKernelGGL(radix_onesweep_kernel<true>, dim3((unsigned)tiles), dim3(kRsThreads), 0, st.stream, src_k, dst_k, src_v, dst_v, n, pass * 8,
 			                   (const uint32_t*)(offsets + pass * kRadix), status + (size_t)pass * tiles * kRadix, tickets + pass, st.async_error_dev, kind, enc, dec);
@@ -439,6 +440,10 @@ static int radix_sort_impl(int kind, const uint32_t* keys_in, const uint32_t* va
 		src_v = dst_v;
 	}
 	return TFHIP_OK;
+}
+
+int radix_sort_low_digits(const uint32_t* keys_in, const uint32_t* vals_in, uint32_t* keys_out, uint32_t* vals_out, uint32_t* keys_tmp, uint32_t* vals_tmp, size_t n, int digits) {
+	return radix_sort_impl(kKeyU32, keys_in, vals_in, keys_out, vals_out, keys_tmp, vals_tmp, n, digits);
 }
 
 }  // namespace tfhip
