@@ -128,6 +128,14 @@ def check(func: str, status: int) -> None:
         raise TFHipError(func, status, msg.decode("utf-8", "replace") if msg else "")
 
 
+_entry_points: dict = {}
+
+
 def call(func: str, *args) -> None:
     """Calls lib.<func>(*args) and raises TFHipError on a non-zero status."""
-    check(func, getattr(load(), func)(*args))
+    fn = _entry_points.get(func)
+    if fn is None:
+        fn = _entry_points[func] = getattr(load(), func)
+    status = fn(*args)
+    if status:
+        check(func, status)

@@ -62,34 +62,12 @@ def _coerce(arr: np.ndarray) -> np.ndarray:
     return np.ascontiguousarray(arr)
 
 
-class DeviceBuffer:
-    """An owned device allocation of `n_words` 32-bit words."""
+class DeviceView:
+    """`n_words` 32-bit words of device memory that something else owns (DeviceBuffer.view)."""
 
-    def __init__(self, n_words: int):
-        if n_words <= 0:
-            raise ValueError("Trying to allocate a tensor with size 0")
-        ptr = C.c_void_p()
-        call("tfhip_malloc", C.byref(ptr), n_words)
-        self.ptr = ptr.value
-        self.n_words = int(n_words)
-        self.owned = True
-
-    @classmethod
-    def view(cls, ptr: int, n_words: int) -> "DeviceBuffer":
-        """A buffer over device memory that something else owns (a tensor of another library): never freed from here.
-        The library's work runs on its own stream, so what fills or reads that memory elsewhere has to be waited for."""
-        if not ptr or ptr % 4 or n_words <= 0:
-            raise ValueError("a view needs a 4-byte aligned device address and at least one word")
-        buf = cls.__new__(cls)
-        buf.ptr, buf.n_words, buf.owned = int(ptr), int(n_words), False
-        return buf
-
-    @classmethod
-    def from_numpy(cls, arr) -> "DeviceBuffer":
-        arr = _coerce(arr)
-        buf = cls(arr.size)
-        buf.write(arr)
-        return buf
+    def __init__(self, ptr: int, n_words: int):
+        self.ptr = ptr
+        self.n_words = n_words
 
     def write(self, arr, offset_words: int = 0) -> None:
         arr = _coerce(arr)
@@ -112,10 +90,39 @@ class DeviceBuffer:
         call("tfhip_fill_u32", self.ptr, word & 0xFFFFFFFF, self.n_words)
 
     def free(self) -> None:
+        """Lets go of the address; the memory stays its owner's."""
+        self.ptr = None
+
+
+class DeviceBuffer(DeviceView):
+    """An owned device allocation of `n_words` 32-bit words."""
+
+    def __init__(self, n_words: int):
+        if n_words <= 0:
+            raise ValueError("Trying to allocate a tensor with size 0")
+        ptr = C.c_void_p()
+        call("tfhip_malloc", C.byref(ptr), n_words)
+        super().__init__(ptr.value, int(n_words))
+
+    @classmethod
+    def from_numpy(cls, arr) -> "DeviceBuffer":
+        arr = _coerce(arr)
+        buf = cls(arr.size)
+        buf.write(arr)
+        return buf
+
+    @staticmethod
+    def view(ptr: int, n_words: int) -> DeviceView:
+        """A buffer over device memory that something else owns (a tensor of another library): never freed from here.
+        The library's work runs on its own stream, so what fills or reads that memory elsewhere has to be waited for."""
+        if not ptr or ptr & 3 or n_words <= 0:
+            raise ValueError("a view needs a 4-byte aligned device address and at least one word")
+        return DeviceView(ptr, n_words)
+
+    def free(self) -> None:
         if self.ptr:
             ptr, self.ptr = self.ptr, None  # the memory is gone even when the call reports an earlier kernel's error
-            if self.owned:
-                call("tfhip_free", ptr)
+            call("tfhip_free", ptr)
 
     def __del__(self):
         try:
@@ -206,7 +213,7 @@ class Kernel:
 
     def launch(self, grid: int, block, buffers, variables=()) -> None:
         bx, by, bz = (list(block) + [1, 1])[:3]
-        ptrs = (C.c_void_p * max(1, len(buffers)))(*[b.ptr if isinstance(b, DeviceBuffer) else b for b in buffers])
+        ptrs = (C.c_void_p * max(1, len(buffers)))(*[b.ptr if isinstance(b, DeviceView) else b for b in buffers])
         words = np.asarray(list(variables), dtype=np.uint32)
         vars_arr = (C.c_uint32 * max(1, len(words)))(*[int(w) for w in words])
         call("tfhip_launch", self.handle, grid, bx, by, bz, ptrs, len(buffers), vars_arr, len(words))
@@ -299,7 +306,7 @@ def sgemm(layout: str, a: DeviceBuffer, b: DeviceBuffer, c: DeviceBuffer, m: int
         call("tfhip_sgemm_fused", {"nn": 0, "nt": 1, "tn": 2}[layout], a.ptr, b.ptr, c.ptr, m, n, k, _EPILOGUES[epilogue], aux.ptr if aux is not None else None)
 
 
-def _words(buf: DeviceBuffer | None, n_words: int, name: str):
+def _words(buf: DeviceView | None, n_words: int, name: str):
     """The address of a buffer that has to hold at least n_words; None stays None."""
     if buf is None:
         return None
@@ -308,8 +315,8 @@ def _words(buf: DeviceBuffer | None, n_words: int, name: str):
     return buf.ptr
 
 
-def layer_norm_rows(x: DeviceBuffer, weight: DeviceBuffer | None, bias: DeviceBuffer | None, y: DeviceBuffer, rows: int, cols: int, eps: float = 1e-5,
-                    mean: DeviceBuffer | None = None, rstd: DeviceBuffer | None = None) -> None:
+def layer_norm_rows(x: DeviceView, weight: DeviceView | None, bias: DeviceView | None, y: DeviceView, rows: int, cols: int, eps: float = 1e-5,
+                    mean: DeviceView | None = None, rstd: DeviceView | None = None) -> None:
     """y = (x - mean) * rstd * weight + bias along every row of x[rows, cols]; mean and rstd receive the rows' statistics,
     which layer_norm_rows_backward takes. weight / bias None: 1 / 0. x may be y."""
     n = rows * cols
@@ -317,8 +324,8 @@ def layer_norm_rows(x: DeviceBuffer, weight: DeviceBuffer | None, bias: DeviceBu
          _words(rstd, rows, "rstd"), rows, cols, eps)
 
 
-def layer_norm_rows_backward(x: DeviceBuffer, dy: DeviceBuffer, weight: DeviceBuffer | None, mean: DeviceBuffer, rstd: DeviceBuffer, rows: int, cols: int,
-                             dx: DeviceBuffer | None = None, dweight: DeviceBuffer | None = None, dbias: DeviceBuffer | None = None) -> None:
+def layer_norm_rows_backward(x: DeviceView, dy: DeviceView, weight: DeviceView | None, mean: DeviceView, rstd: DeviceView, rows: int, cols: int,
+                             dx: DeviceView | None = None, dweight: DeviceView | None = None, dbias: DeviceView | None = None) -> None:
     """The gradients of layer_norm_rows from the upstream gradient dy; any of dx, dweight, dbias that is given. dx may be
     x or dy."""
     n = rows * cols
@@ -326,12 +333,12 @@ def layer_norm_rows_backward(x: DeviceBuffer, dy: DeviceBuffer, weight: DeviceBu
          _words(dx, n, "dx"), _words(dweight, cols, "dweight"), _words(dbias, cols, "dbias"), rows, cols)
 
 
-def embedding_rows(tokens: DeviceBuffer, table: DeviceBuffer, out: DeviceBuffer, n: int, vocab: int, cols: int, scale: float = 1.0) -> None:
+def embedding_rows(tokens: DeviceView, table: DeviceView, out: DeviceView, n: int, vocab: int, cols: int, scale: float = 1.0) -> None:
     """out[i] = scale * table[tokens[i]] for n int32 tokens; zeros for a token outside [0, vocab)."""
     call("tfhip_embedding_rows_f32", _words(tokens, n, "tokens"), _words(table, vocab * cols, "table"), _words(out, n * cols, "out"), n, vocab, cols, scale)
 
 
-def embedding_rows_backward(tokens: DeviceBuffer, dy: DeviceBuffer, dtable: DeviceBuffer, n: int, vocab: int, cols: int, scale: float = 1.0) -> None:
+def embedding_rows_backward(tokens: DeviceView, dy: DeviceView, dtable: DeviceView, n: int, vocab: int, cols: int, scale: float = 1.0) -> None:
     """dtable[v] = scale * the sum of dy[i] over the positions with tokens[i] == v; every row of dtable is written."""
     call("tfhip_embedding_rows_backward_f32", _words(tokens, n, "tokens"), _words(dy, n * cols, "dy"), _words(dtable, vocab * cols, "dtable"), n, vocab, cols, scale)
 
@@ -339,7 +346,7 @@ def embedding_rows_backward(tokens: DeviceBuffer, dy: DeviceBuffer, dtable: Devi
 NEWTON_SCHULZ_QUINTIC = (3.4445, -4.7750, 2.0315)  # drives singular values into about 0.7 .. 1.2 within five steps
 
 
-def newton_schulz(g: DeviceBuffer, out: DeviceBuffer, rows: int, cols: int, steps: int = 5, batch: int = 1, coefficients=NEWTON_SCHULZ_QUINTIC, eps: float = 1e-7) -> None:
+def newton_schulz(g: DeviceView, out: DeviceView, rows: int, cols: int, steps: int = 5, batch: int = 1, coefficients=NEWTON_SCHULZ_QUINTIC, eps: float = 1e-7) -> None:
     """Orthogonalises `batch` matrices [rows, cols] by `steps` Newton-Schulz products. coefficients: (a, b, c) of every
     step, or one such triple per step. g may be out."""
     triples = np.asarray(coefficients, dtype=np.float32)
@@ -353,7 +360,7 @@ def newton_schulz(g: DeviceBuffer, out: DeviceBuffer, rows: int, cols: int, step
 
 
 __all__ = [
-    "initialize", "shutdown", "device_info", "synchronize", "DeviceBuffer", "Event", "Kernel",
+    "initialize", "shutdown", "device_info", "synchronize", "DeviceBuffer", "DeviceView", "Event", "Kernel",
     "reduce_rows", "reduce_cols", "reduce_cols_slabs", "softmax_rows", "log_softmax_rows", "scan_inclusive", "radix_sort_kv", "sgemm",
     "layer_norm_rows", "layer_norm_rows_backward", "embedding_rows", "embedding_rows_backward", "newton_schulz", "NEWTON_SCHULZ_QUINTIC", "TFHipError",
 ]
