@@ -12,72 +12,334 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace tfhip {
 
 constexpr int kLnThreads = 256;
 
-// The sum of v over the group, in every thread. `red` holds one float per wave.
-template <int THREADS>
-__device__ __forceinline__ float group_sum(float v, float* red) {
-	v = wave_reduce(v, OpSum());
-	__syncthreads();
-	if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-	__syncthreads();
-	float t = 0.0f;
+template <int VEC>
+struct LnVec {
+	typedef float type __attribute__((ext_vector_type(VEC)));
+};
+template <>
+struct LnVec<1> {
+	typedef float type;
+};
+
+// E elements of a row per thread of a GROUP, as E / VEC vectors that lie GROUP vectors apart; zero beyond the row.
+template <int GROUP, int E, int VEC>
+__device__ __forceinline__ void load_row(const float* p, float (&v)[E], int lane, int cols) {
+	typedef typename LnVec<VEC>::type Vec;
 #pragma unroll
-	for (int w = 0; w < THREADS / 64; w++) t += red[w];
-	return t;
+	for (int i = 0; i < E / VEC; i++) {
+		const int c = (i * GROUP + lane) * VEC;
+		const Vec t = c < cols ? __builtin_nontemporal_load(reinterpret_cast<const Vec*>(p + c)) : Vec(0.0f);
+		if constexpr (VEC == 1) {
+			v[i] = t;
+		} else {
+#pragma unroll
+			for (int j = 0; j < VEC; j++) v[i * VEC + j] = t[j];
+		}
+	}
+}
+// The same for a vector that every row uses (kept by the caches); `empty` where there is none.
+template <int GROUP, int E, int VEC>
+__device__ __forceinline__ void load_shared(const float* p, float (&v)[E], int lane, int cols, float empty) {
+	typedef typename LnVec<VEC>::type Vec;
+#pragma unroll
+	for (int i = 0; i < E / VEC; i++) {
+		const int c = (i * GROUP + lane) * VEC;
+		const Vec t = p && c < cols ? *reinterpret_cast<const Vec*>(p + c) : Vec(empty);
+		if constexpr (VEC == 1) {
+			v[i] = t;
+		} else {
+#pragma unroll
+			for (int j = 0; j < VEC; j++) v[i * VEC + j] = t[j];
+		}
+	}
+}
+template <int GROUP, int E, int VEC, bool STREAM>
+__device__ __forceinline__ void store_row(float* p, const float (&v)[E], int lane, int cols) {
+	typedef typename LnVec<VEC>::type Vec;
+#pragma unroll
+	for (int i = 0; i < E / VEC; i++) {
+		const int c = (i * GROUP + lane) * VEC;
+		if (c >= cols) continue;
+		Vec t;
+		if constexpr (VEC == 1) {
+			t = v[i];
+		} else {
+#pragma unroll
+			for (int j = 0; j < VEC; j++) t[j] = v[i * VEC + j];
+		}
+		if (STREAM)
+			__builtin_nontemporal_store(t, reinterpret_cast<Vec*>(p + c));
+		else
+			*reinterpret_cast<Vec*>(p + c) = t;
+	}
+}
+// Whether element i of a thread lies inside the row.
+template <int GROUP, int VEC>
+__device__ __forceinline__ bool inside(int i, int lane, int cols) {
+	return (i / VEC * GROUP + lane) * VEC < cols;
 }
 
-// A group per row, the row read three times (from the caches after the first).
-__global__ __launch_bounds__(kLnThreads) void layer_norm_long_kernel(const float* x, const float* __restrict__ weight, const float* __restrict__ bias, float* y, float* __restrict__ mean_out,
-                                                                     float* __restrict__ rstd_out, size_t rows, size_t cols, float eps) {
-	__shared__ float red[kLnThreads / 64];
-	for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
-		const float* px = x + row * cols;
-		float* py = y + row * cols;
-		float sum = 0.0f;
-		for (size_t c = threadIdx.x; c < cols; c += kLnThreads) sum += px[c];
-		const float mean = group_sum<kLnThreads>(sum, red) / (float)cols;
-		float sq = 0.0f;
-		for (size_t c = threadIdx.x; c < cols; c += kLnThreads) {
-			const float d = px[c] - mean;
-			sq += d * d;
-		}
-		const float rstd = 1.0f / sqrtf(group_sum<kLnThreads>(sq, red) / (float)cols + eps);
-		for (size_t c = threadIdx.x; c < cols; c += kLnThreads) py[c] = (px[c] - mean) * rstd * (weight ? weight[c] : 1.0f) + (bias ? bias[c] : 0.0f);
-		if (threadIdx.x == 0) {
-			if (mean_out) mean_out[row] = mean;
-			if (rstd_out) rstd_out[row] = rstd;
+// N sums over the threads of a GROUP at once, in every thread. Up to a wave by exchanges; larger groups (the whole
+// block) through group memory, `red` with room for N * GROUP / 64 floats that no other call in flight uses.
+template <int GROUP, int N>
+__device__ __forceinline__ void group_sums(float (&v)[N], float* red) {
+#pragma unroll
+	for (int off = (GROUP < 64 ? GROUP : 64) / 2; off >= 1; off >>= 1)
+#pragma unroll
+		for (int i = 0; i < N; i++) v[i] += __shfl_xor(v[i], off, 64);
+	if constexpr (GROUP > 64) {
+		if ((threadIdx.x & 63) == 0)
+#pragma unroll
+			for (int i = 0; i < N; i++) red[(threadIdx.x >> 6) * N + i] = v[i];
+		__syncthreads();
+#pragma unroll
+		for (int i = 0; i < N; i++) {
+			float t = 0.0f;
+#pragma unroll
+			for (int w = 0; w < GROUP / 64; w++) t += red[w * N + i];
+			v[i] = t;
 		}
 	}
 }
 
-// dx: a group per row, the row of x and of dy read twice. A thread writes only elements it has read, after the sums:
-// dx may be x or dy.
-__global__ __launch_bounds__(kLnThreads) void layer_norm_long_dx_kernel(const float* x, const float* dy, const float* __restrict__ weight, const float* __restrict__ mean,
-                                                                        const float* __restrict__ rstd, float* dx, size_t rows, size_t cols) {
-	__shared__ float red[kLnThreads / 64];
-	for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
-		const size_t at = row * cols;
-		const float m = mean[row], s = rstd[row];
-		float sum_g = 0.0f, sum_gx = 0.0f;
-		for (size_t c = threadIdx.x; c < cols; c += kLnThreads) {
-			const float g = dy[at + c] * (weight ? weight[c] : 1.0f);
-			sum_g += g;
-			sum_gx += g * ((x[at + c] - m) * s);
+// ---- forward ---------------------------------------------------------------------------------------
+
+// GROUP threads own R rows at a time, each row in registers: one read, one write. Rows of up to 1024 elements take (part
+// of) a wave, so that the sums need no barrier; longer ones a block.
+template <int GROUP, int E, int VEC, int R>
+__global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void layer_norm_kernel(const float* x, const float* __restrict__ weight, const float* __restrict__ bias, float* y,
+                                                                                float* __restrict__ mean_out, float* __restrict__ rstd_out, size_t rows, int cols, float eps) {
+	constexpr int kThreads = GROUP > 256 ? GROUP : 256;
+	__shared__ float red[GROUP > 64 ? 2 * R * GROUP / 64 : 1];
+	const int lane = threadIdx.x % GROUP;
+	const size_t first = ((size_t)blockIdx.x * (kThreads / GROUP) + threadIdx.x / GROUP) * R;
+	float v[R][E], sum[R], sq[R];
+#pragma unroll
+	for (int r = 0; r < R; r++) load_row<GROUP, E, VEC>(x + (first + r < rows ? first + r : rows - 1) * cols, v[r], lane, cols);
+	float w[E], b[E];
+	load_shared<GROUP, E, VEC>(weight, w, lane, cols, 1.0f);
+	load_shared<GROUP, E, VEC>(bias, b, lane, cols, 0.0f);
+#pragma unroll
+	for (int r = 0; r < R; r++) {
+		sum[r] = 0.0f;
+#pragma unroll
+		for (int i = 0; i < E; i++) sum[r] += v[r][i];
+	}
+	group_sums<GROUP, R>(sum, red);
+	const float count = (float)cols;
+#pragma unroll
+	for (int r = 0; r < R; r++) {
+		sum[r] /= count;
+		sq[r] = 0.0f;
+#pragma unroll
+		for (int i = 0; i < E; i++) {
+			v[r][i] -= sum[r];
+			sq[r] += inside<GROUP, VEC>(i, lane, cols) ? v[r][i] * v[r][i] : 0.0f;
 		}
-		const float mean_g = group_sum<kLnThreads>(sum_g, red) / (float)cols;
-		const float mean_gx = group_sum<kLnThreads>(sum_gx, red) / (float)cols;
-		for (size_t c = threadIdx.x; c < cols; c += kLnThreads) {
-			const float g = dy[at + c] * (weight ? weight[c] : 1.0f);
-			const float xhat = (x[at + c] - m) * s;
-			dx[at + c] = s * (g - mean_g - xhat * mean_gx);
+	}
+	group_sums<GROUP, R>(sq, red + (GROUP > 64 ? R * GROUP / 64 : 0));
+#pragma unroll
+	for (int r = 0; r < R; r++) {
+		if (first + r >= rows) break;
+		const float rstd = 1.0f / sqrtf(sq[r] / count + eps);
+#pragma unroll
+		for (int i = 0; i < E; i++) v[r][i] = v[r][i] * rstd * w[i] + b[i];
+		store_row<GROUP, E, VEC, true>(y + (first + r) * cols, v[r], lane, cols);
+		if (lane == 0) {
+			if (mean_out) mean_out[first + r] = sum[r];
+			if (rstd_out) rstd_out[first + r] = rstd;
 		}
 	}
 }
 
-// Partial sums of dw and db: group (tile of 256 columns, slab of rows), one column per thread. partial[slab][2][cols].
+// Rows too long for the registers of a block: cut into segments of kLnSegment. One kernel leaves the sum and the sum
+// of squares about its own mean of every segment, a second joins a row's segments,
+//   mean = sum n_s mean_s / n,   sum of squares = sum (q_s + n_s (mean_s - mean)^2),
+// and normalises one of them: two reads and one write whatever the number of rows.
+constexpr int kLnSegment = 8192, kLnSegmentElements = kLnSegment / kLnThreads;
+
+__global__ __launch_bounds__(kLnThreads) void layer_norm_segment_kernel(const float* __restrict__ x, float2* __restrict__ stats, int cols, int segments) {
+	__shared__ float red[2 * kLnThreads / 64];
+	const size_t row = blockIdx.x / segments;
+	const int c0 = (int)(blockIdx.x % segments) * kLnSegment, count = cols - c0 < kLnSegment ? cols - c0 : kLnSegment;
+	const float* p = x + row * cols + c0;
+	float v[kLnSegmentElements], sum[1] = {0.0f}, sq[1] = {0.0f};
+#pragma unroll
+	for (int i = 0; i < kLnSegmentElements; i++) {
+		const int c = i * kLnThreads + threadIdx.x;
+		v[i] = c < count ? p[c] : 0.0f;
+	}
+#pragma unroll
+	for (int i = 0; i < kLnSegmentElements; i++) sum[0] += v[i];
+	group_sums<kLnThreads, 1>(sum, red);
+	const float mean = sum[0] / (float)count;
+#pragma unroll
+	for (int i = 0; i < kLnSegmentElements; i++) {
+		const float d = v[i] - mean;
+		sq[0] += i * kLnThreads + (int)threadIdx.x < count ? d * d : 0.0f;
+	}
+	group_sums<kLnThreads, 1>(sq, red + kLnThreads / 64);
+	if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(mean, sq[0]);
+}
+
+__global__ __launch_bounds__(kLnThreads) void layer_norm_apply_kernel(const float* x, const float* __restrict__ weight, const float* __restrict__ bias, float* y, float* __restrict__ mean_out,
+                                                                      float* __restrict__ rstd_out, const float2* __restrict__ stats, int cols, int segments, float eps) {
+	__shared__ float red[2 * kLnThreads / 64];
+	const size_t row = blockIdx.x / segments;
+	const int segment = (int)(blockIdx.x % segments), c0 = segment * kLnSegment, count = cols - c0 < kLnSegment ? cols - c0 : kLnSegment;
+	const float2* st = stats + row * segments;
+	float sum[1] = {0.0f}, sq[1] = {0.0f};
+	for (int s = threadIdx.x; s < segments; s += kLnThreads) sum[0] += st[s].x * (float)(cols - s * kLnSegment < kLnSegment ? cols - s * kLnSegment : kLnSegment);
+	group_sums<kLnThreads, 1>(sum, red);
+	const float mean = sum[0] / (float)cols;
+	for (int s = threadIdx.x; s < segments; s += kLnThreads) {
+		const float d = st[s].x - mean;
+		sq[0] += st[s].y + d * d * (float)(cols - s * kLnSegment < kLnSegment ? cols - s * kLnSegment : kLnSegment);
+	}
+	group_sums<kLnThreads, 1>(sq, red + kLnThreads / 64);
+	const float rstd = 1.0f / sqrtf(sq[0] / (float)cols + eps);
+	const float* px = x + row * cols + c0;
+	float* py = y + row * cols + c0;
+	for (int c = threadIdx.x; c < count; c += kLnThreads) py[c] = (px[c] - mean) * rstd * (weight ? weight[c0 + c] : 1.0f) + (bias ? bias[c0 + c] : 0.0f);
+	if (segment == 0 && threadIdx.x == 0) {
+		if (mean_out) mean_out[row] = mean;
+		if (rstd_out) rstd_out[row] = rstd;
+	}
+}
+
+// ---- backward --------------------------------------------------------------------------------------
+
+// As the forward kernel, but a group stays and takes rows in turn (`step` groups in all): the column sums of dy xhat and
+// dy of its rows stay in its registers and leave once, partial[block][2][cols], after the groups of a block have added
+// theirs up in group memory. Each of x and dy is read once, dx written once.
+template <int GROUP, int E, int VEC, int R>
+__global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void layer_norm_backward_kernel(const float* x, const float* dy, const float* __restrict__ weight, const float* __restrict__ mean,
+                                                                                        const float* __restrict__ rstd, float* dx, float* __restrict__ partial, size_t rows, int cols) {
+	constexpr int kThreads = GROUP > 256 ? GROUP : 256, kGroups = kThreads / GROUP;
+	// for the sums of a large group (two in turn, so that one barrier a row is enough), then for the join of the groups' columns
+	__shared__ float red[GROUP > 64 ? 4 * R * GROUP / 64 : kGroups * GROUP * E];
+	const int lane = threadIdx.x % GROUP, group = threadIdx.x / GROUP;
+	float w[E], sum_dw[E], sum_db[E];
+	load_shared<GROUP, E, VEC>(weight, w, lane, cols, 1.0f);
+#pragma unroll
+	for (int i = 0; i < E; i++) sum_dw[i] = sum_db[i] = 0.0f;
+	const size_t step = (size_t)gridDim.x * kGroups * R;
+	const float count = (float)cols;
+	int turn = 0;
+	for (size_t first = ((size_t)blockIdx.x * kGroups + group) * R; first < rows; first += step) {
+		float vx[R][E], vdy[R][E], m[R], s[R], sums[2 * R];
+#pragma unroll
+		for (int r = 0; r < R; r++) {
+			const size_t row = first + r < rows ? first + r : rows - 1;
+			m[r] = mean[row];
+			s[r] = rstd[row];
+			load_row<GROUP, E, VEC>(x + row * cols, vx[r], lane, cols);
+			load_row<GROUP, E, VEC>(dy + row * cols, vdy[r], lane, cols);
+		}
+#pragma unroll
+		for (int r = 0; r < R; r++) {
+			sums[2 * r] = sums[2 * r + 1] = 0.0f;
+			const bool real = R == 1 || first + r < rows;
+#pragma unroll
+			for (int i = 0; i < E; i++) {
+				vx[r][i] = (vx[r][i] - m[r]) * s[r];  // xhat; beyond the row dy is 0, and 0 times a finite number adds nothing
+				if (!inside<GROUP, VEC>(i, lane, cols)) vx[r][i] = 0.0f;
+				if (real) {
+					sum_dw[i] += vdy[r][i] * vx[r][i];
+					sum_db[i] += vdy[r][i];
+				}
+				vdy[r][i] *= w[i];
+				sums[2 * r] += vdy[r][i];
+				sums[2 * r + 1] += vdy[r][i] * vx[r][i];
+			}
+		}
+		if (dx) {
+			group_sums<GROUP, 2 * R>(sums, red + (GROUP > 64 ? turn * 2 * R * GROUP / 64 : 0));
+			turn ^= 1;
+#pragma unroll
+			for (int r = 0; r < R; r++) {
+				if (first + r >= rows) break;
+				const float mg = sums[2 * r] / count, mgx = sums[2 * r + 1] / count;
+#pragma unroll
+				for (int i = 0; i < E; i++) vdy[r][i] = s[r] * (vdy[r][i] - mg - vx[r][i] * mgx);
+				store_row<GROUP, E, VEC, true>(dx + (first + r) * cols, vdy[r], lane, cols);
+			}
+		}
+	}
+	if (!partial) return;
+	partial += (size_t)blockIdx.x * 2 * cols;
+	if constexpr (kGroups > 1) {
+#pragma unroll
+		for (int which = 0; which < 2; which++) {
+			__syncthreads();
+#pragma unroll
+			for (int i = 0; i < E; i++) red[(group * E + i) * GROUP + lane] = which ? sum_db[i] : sum_dw[i];
+			__syncthreads();
+			if (group == 0) {
+#pragma unroll
+				for (int i = 0; i < E; i++) {
+					float t = red[i * GROUP + lane];
+					for (int g = 1; g < kGroups; g++) t += red[(g * E + i) * GROUP + lane];
+					if (which)
+						sum_db[i] = t;
+					else
+						sum_dw[i] = t;
+				}
+			}
+		}
+		if (group != 0) return;
+	}
+	store_row<GROUP, E, VEC, false>(partial, sum_dw, lane, cols);
+	store_row<GROUP, E, VEC, false>(partial + cols, sum_db, lane, cols);
+}
+
+// dx of rows cut into segments: the two sums of every segment, then the join and dx of one segment. A thread writes only
+// elements that it alone reads, after reading them.
+__global__ __launch_bounds__(kLnThreads) void layer_norm_segment_sums_kernel(const float* __restrict__ x, const float* __restrict__ dy, const float* __restrict__ weight,
+                                                                             const float* __restrict__ mean, const float* __restrict__ rstd, float2* __restrict__ stats, int cols, int segments) {
+	__shared__ float red[2 * kLnThreads / 64];
+	const size_t row = blockIdx.x / segments;
+	const int c0 = (int)(blockIdx.x % segments) * kLnSegment, count = cols - c0 < kLnSegment ? cols - c0 : kLnSegment;
+	const float *px = x + row * cols + c0, *pdy = dy + row * cols + c0;
+	const float m = mean[row], s = rstd[row];
+	float sums[2] = {0.0f, 0.0f};
+#pragma unroll 8
+	for (int i = 0; i < kLnSegmentElements; i++) {
+		const int c = i * kLnThreads + threadIdx.x;
+		const float g = c < count ? pdy[c] * (weight ? weight[c0 + c] : 1.0f) : 0.0f, xhat = c < count ? (px[c] - m) * s : 0.0f;
+		sums[0] += g;
+		sums[1] += g * xhat;
+	}
+	group_sums<kLnThreads, 2>(sums, red);
+	if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(sums[0], sums[1]);
+}
+
+__global__ __launch_bounds__(kLnThreads) void layer_norm_segment_dx_kernel(const float* x, const float* dy, const float* __restrict__ weight, const float* __restrict__ mean,
+                                                                           const float* __restrict__ rstd, float* dx, const float2* __restrict__ stats, int cols, int segments) {
+	__shared__ float red[2 * kLnThreads / 64];
+	const size_t row = blockIdx.x / segments, at = row * cols;
+	const int c0 = (int)(blockIdx.x % segments) * kLnSegment, c1 = cols - c0 < kLnSegment ? cols : c0 + kLnSegment;
+	float sums[2] = {0.0f, 0.0f};
+	for (int k = threadIdx.x; k < segments; k += kLnThreads) {
+		const float2 t = stats[row * segments + k];
+		sums[0] += t.x;
+		sums[1] += t.y;
+	}
+	group_sums<kLnThreads, 2>(sums, red);
+	const float m = mean[row], s = rstd[row], mg = sums[0] / (float)cols, mgx = sums[1] / (float)cols;
+	for (int c = c0 + threadIdx.x; c < c1; c += kLnThreads) {
+		const float g = dy[at + c] * (weight ? weight[c] : 1.0f), xhat = (x[at + c] - m) * s;
+		dx[at + c] = s * (g - mg - xhat * mgx);
+	}
+}
+
+// Partial sums of dw and db for such rows: group (tile of 256 columns, slab of rows), one column per thread.
 __global__ __launch_bounds__(kLnThreads) void layer_norm_dweight_kernel(const float* __restrict__ x, const float* __restrict__ dy, const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                         float* __restrict__ partial, size_t rows, size_t cols, size_t rows_per_slab, unsigned col_tiles) {
 	const size_t c = (size_t)(blockIdx.x % col_tiles) * kLnThreads + threadIdx.x;
@@ -85,6 +347,7 @@ __global__ __launch_bounds__(kLnThreads) void layer_norm_dweight_kernel(const fl
 	if (c >= cols) return;
 	const size_t r0 = slab * rows_per_slab, r1 = r0 + rows_per_slab < rows ? r0 + rows_per_slab : rows;
 	float dw = 0.0f, db = 0.0f;
+#pragma unroll 4
 	for (size_t r = r0; r < r1; r++) {
 		const float d = dy[r * cols + c];
 		dw += d * ((x[r * cols + c] - mean[r]) * rstd[r]);
@@ -94,16 +357,147 @@ __global__ __launch_bounds__(kLnThreads) void layer_norm_dweight_kernel(const fl
 	partial[(slab * 2 + 1) * cols + c] = db;
 }
 
-__global__ __launch_bounds__(kLnThreads) void layer_norm_fold_kernel(const float* __restrict__ partial, float* __restrict__ dweight, float* __restrict__ dbias, size_t slabs, size_t cols) {
-	const size_t c = (size_t)blockIdx.x * kLnThreads + threadIdx.x;
-	if (c >= cols) return;
-	float dw = 0.0f, db = 0.0f;
-	for (size_t k = 0; k < slabs; k++) {
-		dw += partial[(k * 2) * cols + c];
-		db += partial[(k * 2 + 1) * cols + c];
+// The sum of the partial results, in a fixed order: a block of 16 waves per 64 of the 2 cols columns, wave w the parts
+// w, w + 16, ..., then the waves' sums in the order of the waves.
+constexpr int kFoldWaves = 16;
+__global__ __launch_bounds__(kFoldWaves * 64) void layer_norm_fold_kernel(const float* __restrict__ partial, float* __restrict__ dweight, float* __restrict__ dbias, size_t parts, size_t cols) {
+	__shared__ float red[kFoldWaves][64];
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+	const size_t c = (size_t)blockIdx.x * 64 + lane, width = 2 * cols;
+	float sum = 0.0f;
+	if (c < width) {
+		size_t k = wave;
+		for (; k + 7 * kFoldWaves < parts; k += 8 * kFoldWaves) {
+			float t[8];
+#pragma unroll
+			for (int u = 0; u < 8; u++) t[u] = partial[(k + u * kFoldWaves) * width + c];
+#pragma unroll
+			for (int u = 0; u < 8; u++) sum += t[u];
+		}
+		for (; k < parts; k += kFoldWaves) sum += partial[k * width + c];
 	}
-	if (dweight) dweight[c] = dw;
-	if (dbias) dbias[c] = db;
+	red[wave][lane] = sum;
+	__syncthreads();
+	if (wave != 0 || c >= width) return;
+#pragma unroll
+	for (int w = 1; w < kFoldWaves; w++) sum += red[w][lane];
+	float* to = c < cols ? dweight : dbias;
+	if (to) to[c < cols ? c : c - cols] = sum;
+}
+
+// ---- which kernel ------------------------------------------------------------------------------------
+
+constexpr size_t kLnMostInRegisters = 16384;
+
+// Calls f with (threads of a row, elements of a thread, rows at a time) as constants: the smallest group that holds the
+// row with four elements a thread up to a wave, then more elements, then a block. Several short rows at a time hide the
+// exchanges of their sums behind each other.
+template <int VEC, class F>
+static void with_row_group(size_t cols, F f) {
+	using std::integral_constant;
+#define TFHIP_LN_CASE(GROUP, E, R) f(integral_constant<int, GROUP>(), integral_constant<int, E>(), integral_constant<int, VEC>(), integral_constant<int, R>())
+	if (cols <= 32) TFHIP_LN_CASE(8, 4, 2);
+	else if (cols <= 64) TFHIP_LN_CASE(16, 4, 2);
+	else if (cols <= 128) TFHIP_LN_CASE(32, 4, 4);
+	else if (cols <= 256) TFHIP_LN_CASE(64, 4, 4);
+	else if (cols <= 512) TFHIP_LN_CASE(64, 8, 2);
+	else if (cols <= 1024) TFHIP_LN_CASE(64, 16, 1);
+	else if (cols <= 2048) TFHIP_LN_CASE(256, 8, 1);
+	else if (cols <= 4096) TFHIP_LN_CASE(256, 16, 1);
+	else if (cols <= 8192) TFHIP_LN_CASE(1024, 8, 1);
+	else TFHIP_LN_CASE(1024, 16, 1);
+#undef TFHIP_LN_CASE
+}
+
+static bool aligned16(const void* a, const void* b, const void* c, const void* d) { return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) & 15) == 0; }
+
+template <int VEC>
+static int layer_norm_forward(const float* x, const float* weight, const float* bias, float* y, float* mean, float* rstd, size_t rows, size_t cols, float eps) {
+	State& s = state();
+	with_row_group<VEC>(cols, [&](auto group, auto e, auto vec, auto r) {
+		constexpr int kGroup = decltype(group)::value, kThreads = kGroup > 256 ? kGroup : 256, kRows = kThreads / kGroup * decltype(r)::value;
+		hipLaunchKernelGGL((layer_norm_kernel<kGroup, decltype(e)::value, decltype(vec)::value, decltype(r)::value>), dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(kThreads), 0, s.stream, x,
+		                   weight, bias, y, mean, rstd, rows, (int)cols, eps);
+	});
+	TFHIP_CHECK_LAUNCH();
+	return TFHIP_OK;
+}
+
+static int launch_fold(const float* partial, float* dweight, float* dbias, size_t parts, size_t cols) {
+	hipLaunchKernelGGL(layer_norm_fold_kernel, dim3((unsigned)((2 * cols + 63) / 64)), dim3(kFoldWaves * 64), 0, state().stream, partial, dweight, dbias, parts, cols);
+	TFHIP_CHECK_LAUNCH();
+	return TFHIP_OK;
+}
+
+template <int VEC>
+static int layer_norm_backward(const float* x, const float* dy, const float* weight, const float* mean, const float* rstd, float* dx, float* dweight, float* dbias, size_t rows, size_t cols) {
+	State& s = state();
+	int rc = TFHIP_OK;
+	with_row_group<VEC>(cols, [&](auto group, auto e, auto vec, auto r) {
+		constexpr int kGroup = decltype(group)::value, kThreads = kGroup > 256 ? kGroup : 256, kRows = kThreads / kGroup * decltype(r)::value;
+		// as many blocks as stay resident, 1024 threads a unit
+		const size_t most = (size_t)s.compute_units * 1024 / kThreads, want = (rows + kRows - 1) / kRows, blocks = want < most ? want : most;
+		float* partial = nullptr;
+		if (dweight || dbias) {
+			partial = (float*)scratch(blocks * 2 * cols * sizeof(float));
+			if (!partial) {
+				rc = TFHIP_ERR_HIP;
+				return;
+			}
+		}
+		hipLaunchKernelGGL((layer_norm_backward_kernel<kGroup, decltype(e)::value, decltype(vec)::value, decltype(r)::value>), dim3((unsigned)blocks), dim3(kThreads), 0, s.stream, x, dy, weight,
+		                   mean, rstd, dx, partial, rows, (int)cols);
+		const hipError_t err = hipGetLastError();
+		if (err != hipSuccess)
+			rc = fail_hip(err, "layer norm backward launch");
+		else if (partial)
+			rc = launch_fold(partial, dweight, dbias, blocks, cols);
+	});
+	return rc;
+}
+
+static int layer_norm_long_backward(const float* x, const float* dy, const float* weight, const float* mean, const float* rstd, float* dx, float* dweight, float* dbias, size_t rows, size_t cols) {
+	State& s = state();
+	const size_t segments = (cols + kLnSegment - 1) / kLnSegment, col_tiles = (cols + kLnThreads - 1) / kLnThreads;
+	if (rows * segments > 0x7FFFFFFF) return fail(TFHIP_ERR_ARG, "layer norm of %zu x %zu is too large", rows, cols);
+	size_t slabs = (size_t)s.compute_units * 8 / col_tiles;
+	if (slabs > (rows + 15) / 16) slabs = (rows + 15) / 16;
+	if (slabs < 1) slabs = 1;
+	const size_t per = (rows + slabs - 1) / slabs;
+	slabs = (rows + per - 1) / per;
+	const size_t stats_bytes = (rows * segments * sizeof(float2) + 255) & ~size_t(255);
+	char* base = (char*)scratch(stats_bytes + slabs * 2 * cols * sizeof(float));
+	if (!base) return TFHIP_ERR_HIP;
+	float2* stats = (float2*)base;
+	float* partial = (float*)(base + stats_bytes);
+	if (dweight || dbias) {  // before dx, which may overwrite x or dy
+		hipLaunchKernelGGL(layer_norm_dweight_kernel, dim3((unsigned)(col_tiles * slabs)), dim3(kLnThreads), 0, s.stream, x, dy, mean, rstd, partial, rows, cols, per, (unsigned)col_tiles);
+		TFHIP_CHECK_LAUNCH();
+		const int rc = launch_fold(partial, dweight, dbias, slabs, cols);
+		if (rc) return rc;
+	}
+	if (dx) {
+		const dim3 grid((unsigned)(rows * segments)), block(kLnThreads);
+		hipLaunchKernelGGL(layer_norm_segment_sums_kernel, grid, block, 0, s.stream, x, dy, weight, mean, rstd, stats, (int)cols, (int)segments);
+		TFHIP_CHECK_LAUNCH();
+		hipLaunchKernelGGL(layer_norm_segment_dx_kernel, grid, block, 0, s.stream, x, dy, weight, mean, rstd, dx, (const float2*)stats, (int)cols, (int)segments);
+		TFHIP_CHECK_LAUNCH();
+	}
+	return TFHIP_OK;
+}
+
+static int layer_norm_long_forward(const float* x, const float* weight, const float* bias, float* y, float* mean, float* rstd, size_t rows, size_t cols, float eps) {
+	State& s = state();
+	const size_t segments = (cols + kLnSegment - 1) / kLnSegment;
+	if (rows * segments > 0x7FFFFFFF) return fail(TFHIP_ERR_ARG, "layer norm of %zu x %zu is too large", rows, cols);
+	float2* stats = (float2*)scratch(rows * segments * sizeof(float2));
+	if (!stats) return TFHIP_ERR_HIP;
+	const dim3 grid((unsigned)(rows * segments)), block(kLnThreads);
+	hipLaunchKernelGGL(layer_norm_segment_kernel, grid, block, 0, s.stream, x, stats, (int)cols, (int)segments);
+	TFHIP_CHECK_LAUNCH();
+	hipLaunchKernelGGL(layer_norm_apply_kernel, grid, block, 0, s.stream, x, weight, bias, y, mean, rstd, (const float2*)stats, (int)cols, (int)segments, eps);
+	TFHIP_CHECK_LAUNCH();
+	return TFHIP_OK;
 }
 
 static int check_extent(size_t rows, size_t cols) {
@@ -147,11 +541,9 @@ extern "C" int tfhip_layer_norm_rows_f32(const float* x, const float* weight, co
 	if (rc) return rc;
 	TFHIP_REQUIRE_INIT();
 	TFHIP_HOLD_DEVICE();
-	State& s = state();
-	const size_t groups = rows < 65536 ? rows : 65536;
-	hipLaunchKernelGGL(layer_norm_long_kernel, dim3((unsigned)groups), dim3(kLnThreads), 0, s.stream, x, weight, bias, y, mean, rstd, rows, cols, eps);
-	TFHIP_CHECK_LAUNCH();
-	return TFHIP_OK;
+	if (cols > kLnMostInRegisters) return layer_norm_long_forward(x, weight, bias, y, mean, rstd, rows, cols, eps);
+	if (cols % 4 == 0 && aligned16(x, y, weight, bias)) return layer_norm_forward<4>(x, weight, bias, y, mean, rstd, rows, cols, eps);
+	return layer_norm_forward<1>(x, weight, bias, y, mean, rstd, rows, cols, eps);
 }
 
 extern "C" int tfhip_layer_norm_rows_backward_f32(const float* x, const float* dy, const float* weight, const float* mean, const float* rstd, float* dx, float* dweight, float* dbias, size_t rows,
@@ -166,30 +558,12 @@ extern "C" int tfhip_layer_norm_rows_backward_f32(const float* x, const float* d
 	if (rc) return rc;
 	TFHIP_REQUIRE_INIT();
 	TFHIP_HOLD_DEVICE();
-	State& s = state();
 	if (rows == 0) {
 		if (dweight && (rc = tfhip_fill_u32(dweight, 0u, cols))) return rc;
 		if (dbias && (rc = tfhip_fill_u32(dbias, 0u, cols))) return rc;
 		return TFHIP_OK;
 	}
-	if (dweight || dbias) {  // before dx, which may overwrite x or dy
-		const size_t col_tiles = (cols + kLnThreads - 1) / kLnThreads;
-		size_t slabs = (size_t)s.compute_units * 8 / col_tiles;
-		if (slabs > (rows + 15) / 16) slabs = (rows + 15) / 16;
-		if (slabs < 1) slabs = 1;
-		const size_t per = (rows + slabs - 1) / slabs;
-		slabs = (rows + per - 1) / per;
-		float* partial = (float*)scratch(slabs * 2 * cols * sizeof(float));
-		if (!partial) return TFHIP_ERR_HIP;
-		hipLaunchKernelGGL(layer_norm_dweight_kernel, dim3((unsigned)(col_tiles * slabs)), dim3(kLnThreads), 0, s.stream, x, dy, mean, rstd, partial, rows, cols, per, (unsigned)col_tiles);
-		TFHIP_CHECK_LAUNCH();
-		hipLaunchKernelGGL(layer_norm_fold_kernel, dim3((unsigned)col_tiles), dim3(kLnThreads), 0, s.stream, (const float*)partial, dweight, dbias, slabs, cols);
-		TFHIP_CHECK_LAUNCH();
-	}
-	if (dx) {
-		const size_t groups = rows < 65536 ? rows : 65536;
-		hipLaunchKernelGGL(layer_norm_long_dx_kernel, dim3((unsigned)groups), dim3(kLnThreads), 0, s.stream, x, dy, weight, mean, rstd, dx, rows, cols);
-		TFHIP_CHECK_LAUNCH();
-	}
-	return TFHIP_OK;
+	if (cols > kLnMostInRegisters) return layer_norm_long_backward(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, cols);
+	if (cols % 4 == 0 && aligned16(x, dy, weight, dx)) return layer_norm_backward<4>(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, cols);
+	return layer_norm_backward<1>(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, cols);
 }
