@@ -164,17 +164,14 @@ __global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void layer_norm_kernel(c
 // and normalises one of them: two reads and one write whatever the number of rows.
 constexpr int kLnSegment = 8192, kLnSegmentElements = kLnSegment / kLnThreads;
 
+template <int VEC>
 __global__ __launch_bounds__(kLnThreads) void layer_norm_segment_kernel(const float* __restrict__ x, float2* __restrict__ stats, int cols, int segments) {
 	__shared__ float red[2 * kLnThreads / 64];
 	const size_t row = blockIdx.x / segments;
 	const int c0 = (int)(blockIdx.x % segments) * kLnSegment, count = cols - c0 < kLnSegment ? cols - c0 : kLnSegment;
 	const float* p = x + row * cols + c0;
 	float v[kLnSegmentElements], sum[1] = {0.0f}, sq[1] = {0.0f};
-#pragma unroll
-	for (int i = 0; i < kLnSegmentElements; i++) {
-		const int c = i * kLnThreads + threadIdx.x;
-		v[i] = c < count ? p[c] : 0.0f;
-	}
+	load_shared<kLnThreads, kLnSegmentElements, VEC>(p, v, threadIdx.x, count, 0.0f);
 #pragma unroll
 	for (int i = 0; i < kLnSegmentElements; i++) sum[0] += v[i];
 	group_sums<kLnThreads, 1>(sum, red);
@@ -182,17 +179,20 @@ __global__ __launch_bounds__(kLnThreads) void layer_norm_segment_kernel(const fl
 #pragma unroll
 	for (int i = 0; i < kLnSegmentElements; i++) {
 		const float d = v[i] - mean;
-		sq[0] += i * kLnThreads + (int)threadIdx.x < count ? d * d : 0.0f;
+		sq[0] += inside<kLnThreads, VEC>(i, threadIdx.x, count) ? d * d : 0.0f;
 	}
 	group_sums<kLnThreads, 1>(sq, red + kLnThreads / 64);
 	if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(mean, sq[0]);
 }
 
+template <int VEC>
 __global__ __launch_bounds__(kLnThreads) void layer_norm_apply_kernel(const float* x, const float* __restrict__ weight, const float* __restrict__ bias, float* y, float* __restrict__ mean_out,
                                                                       float* __restrict__ rstd_out, const float2* __restrict__ stats, int cols, int segments, float eps) {
 	__shared__ float red[2 * kLnThreads / 64];
 	const size_t row = blockIdx.x / segments;
 	const int segment = (int)(blockIdx.x % segments), c0 = segment * kLnSegment, count = cols - c0 < kLnSegment ? cols - c0 : kLnSegment;
+	float v[kLnSegmentElements];
+	load_shared<kLnThreads, kLnSegmentElements, VEC>(x + row * cols + c0, v, threadIdx.x, count, 0.0f);
 	const float2* st = stats + row * segments;
 	float sum[1] = {0.0f}, sq[1] = {0.0f};
 	for (int s = threadIdx.x; s < segments; s += kLnThreads) sum[0] += st[s].x * (float)(cols - s * kLnSegment < kLnSegment ? cols - s * kLnSegment : kLnSegment);
@@ -204,9 +204,14 @@ __global__ __launch_bounds__(kLnThreads) void layer_norm_apply_kernel(const floa
 	}
 	group_sums<kLnThreads, 1>(sq, red + kLnThreads / 64);
 	const float rstd = 1.0f / sqrtf(sq[0] / (float)cols + eps);
-	const float* px = x + row * cols + c0;
-	float* py = y + row * cols + c0;
-	for (int c = threadIdx.x; c < count; c += kLnThreads) py[c] = (px[c] - mean) * rstd * (weight ? weight[c0 + c] : 1.0f) + (bias ? bias[c0 + c] : 0.0f);
+	float w[kLnSegmentElements];
+	load_shared<kLnThreads, kLnSegmentElements, VEC>(weight ? weight + c0 : nullptr, w, threadIdx.x, count, 1.0f);
+#pragma unroll
+	for (int i = 0; i < kLnSegmentElements; i++) v[i] = (v[i] - mean) * rstd * w[i];
+	load_shared<kLnThreads, kLnSegmentElements, VEC>(bias ? bias + c0 : nullptr, w, threadIdx.x, count, 0.0f);
+#pragma unroll
+	for (int i = 0; i < kLnSegmentElements; i++) v[i] += w[i];
+	store_row<kLnThreads, kLnSegmentElements, VEC, true>(y + row * cols + c0, v, threadIdx.x, count);
 	if (segment == 0 && threadIdx.x == 0) {
 		if (mean_out) mean_out[row] = mean;
 		if (rstd_out) rstd_out[row] = rstd;
@@ -301,30 +306,38 @@ __global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void layer_norm_backward
 
 // dx of rows cut into segments: the two sums of every segment, then the join and dx of one segment. A thread writes only
 // elements that it alone reads, after reading them.
+template <int VEC>
 __global__ __launch_bounds__(kLnThreads) void layer_norm_segment_sums_kernel(const float* __restrict__ x, const float* __restrict__ dy, const float* __restrict__ weight,
                                                                              const float* __restrict__ mean, const float* __restrict__ rstd, float2* __restrict__ stats, int cols, int segments) {
 	__shared__ float red[2 * kLnThreads / 64];
 	const size_t row = blockIdx.x / segments;
 	const int c0 = (int)(blockIdx.x % segments) * kLnSegment, count = cols - c0 < kLnSegment ? cols - c0 : kLnSegment;
-	const float *px = x + row * cols + c0, *pdy = dy + row * cols + c0;
 	const float m = mean[row], s = rstd[row];
 	float sums[2] = {0.0f, 0.0f};
-#pragma unroll 8
+	float vx[kLnSegmentElements], vdy[kLnSegmentElements], w[kLnSegmentElements];
+	load_shared<kLnThreads, kLnSegmentElements, VEC>(x + row * cols + c0, vx, threadIdx.x, count, 0.0f);
+	load_shared<kLnThreads, kLnSegmentElements, VEC>(dy + row * cols + c0, vdy, threadIdx.x, count, 0.0f);
+	load_shared<kLnThreads, kLnSegmentElements, VEC>(weight ? weight + c0 : nullptr, w, threadIdx.x, count, 1.0f);
+#pragma unroll
 	for (int i = 0; i < kLnSegmentElements; i++) {
-		const int c = i * kLnThreads + threadIdx.x;
-		const float g = c < count ? pdy[c] * (weight ? weight[c0 + c] : 1.0f) : 0.0f, xhat = c < count ? (px[c] - m) * s : 0.0f;
+		const float g = vdy[i] * w[i];
 		sums[0] += g;
-		sums[1] += g * xhat;
+		sums[1] += inside<kLnThreads, VEC>(i, threadIdx.x, count) ? g * ((vx[i] - m) * s) : 0.0f;
 	}
 	group_sums<kLnThreads, 2>(sums, red);
 	if (threadIdx.x == 0) stats[blockIdx.x] = make_float2(sums[0], sums[1]);
 }
 
+template <int VEC>
 __global__ __launch_bounds__(kLnThreads) void layer_norm_segment_dx_kernel(const float* x, const float* dy, const float* __restrict__ weight, const float* __restrict__ mean,
                                                                            const float* __restrict__ rstd, float* dx, const float2* __restrict__ stats, int cols, int segments) {
 	__shared__ float red[2 * kLnThreads / 64];
-	const size_t row = blockIdx.x / segments, at = row * cols;
-	const int c0 = (int)(blockIdx.x % segments) * kLnSegment, c1 = cols - c0 < kLnSegment ? cols : c0 + kLnSegment;
+	const size_t row = blockIdx.x / segments;
+	const int c0 = (int)(blockIdx.x % segments) * kLnSegment, count = cols - c0 < kLnSegment ? cols - c0 : kLnSegment;
+	float vx[kLnSegmentElements], vdy[kLnSegmentElements], w[kLnSegmentElements];
+	load_shared<kLnThreads, kLnSegmentElements, VEC>(x + row * cols + c0, vx, threadIdx.x, count, 0.0f);
+	load_shared<kLnThreads, kLnSegmentElements, VEC>(dy + row * cols + c0, vdy, threadIdx.x, count, 0.0f);
+	load_shared<kLnThreads, kLnSegmentElements, VEC>(weight ? weight + c0 : nullptr, w, threadIdx.x, count, 1.0f);
 	float sums[2] = {0.0f, 0.0f};
 	for (int k = threadIdx.x; k < segments; k += kLnThreads) {
 		const float2 t = stats[row * segments + k];
@@ -333,28 +346,29 @@ __global__ __launch_bounds__(kLnThreads) void layer_norm_segment_dx_kernel(const
 	}
 	group_sums<kLnThreads, 2>(sums, red);
 	const float m = mean[row], s = rstd[row], mg = sums[0] / (float)cols, mgx = sums[1] / (float)cols;
-	for (int c = c0 + threadIdx.x; c < c1; c += kLnThreads) {
-		const float g = dy[at + c] * (weight ? weight[c] : 1.0f), xhat = (x[at + c] - m) * s;
-		dx[at + c] = s * (g - mg - xhat * mgx);
-	}
+#pragma unroll
+	for (int i = 0; i < kLnSegmentElements; i++) vx[i] = s * (vdy[i] * w[i] - mg - (vx[i] - m) * s * mgx);
+	store_row<kLnThreads, kLnSegmentElements, VEC, true>(dx + row * cols + c0, vx, threadIdx.x, count);
 }
 
-// Partial sums of dw and db for such rows: group (tile of 256 columns, slab of rows), one column per thread.
+// Partial sums of dw and db for such rows: group (tile of 256 VEC columns, slab of rows), VEC columns per thread.
+template <int VEC>
 __global__ __launch_bounds__(kLnThreads) void layer_norm_dweight_kernel(const float* __restrict__ x, const float* __restrict__ dy, const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                         float* __restrict__ partial, size_t rows, size_t cols, size_t rows_per_slab, unsigned col_tiles) {
-	const size_t c = (size_t)(blockIdx.x % col_tiles) * kLnThreads + threadIdx.x;
+	typedef typename LnVec<VEC>::type Vec;
+	const size_t c = ((size_t)(blockIdx.x % col_tiles) * kLnThreads + threadIdx.x) * VEC;
 	const size_t slab = blockIdx.x / col_tiles;
 	if (c >= cols) return;
 	const size_t r0 = slab * rows_per_slab, r1 = r0 + rows_per_slab < rows ? r0 + rows_per_slab : rows;
-	float dw = 0.0f, db = 0.0f;
-#pragma unroll 4
+	Vec dw = Vec(0.0f), db = Vec(0.0f);
+#pragma unroll 8
 	for (size_t r = r0; r < r1; r++) {
-		const float d = dy[r * cols + c];
-		dw += d * ((x[r * cols + c] - mean[r]) * rstd[r]);
+		const Vec d = *reinterpret_cast<const Vec*>(dy + r * cols + c), v = *reinterpret_cast<const Vec*>(x + r * cols + c);
+		dw += d * ((v - mean[r]) * rstd[r]);
 		db += d;
 	}
-	partial[(slab * 2) * cols + c] = dw;
-	partial[(slab * 2 + 1) * cols + c] = db;
+	*reinterpret_cast<Vec*>(partial + (slab * 2) * cols + c) = dw;
+	*reinterpret_cast<Vec*>(partial + (slab * 2 + 1) * cols + c) = db;
 }
 
 // The sum of the partial results, in a fixed order: a block of 16 waves per 64 of the 2 cols columns, wave w the parts
@@ -403,8 +417,8 @@ static void with_row_group(size_t cols, F f) {
 	else if (cols <= 512) TFHIP_LN_CASE(64, 8, 2);
 	else if (cols <= 1024) TFHIP_LN_CASE(64, 16, 1);
 	else if (cols <= 2048) TFHIP_LN_CASE(256, 8, 1);
-	else if (cols <= 4096) TFHIP_LN_CASE(256, 16, 1);
-	else if (cols <= 8192) TFHIP_LN_CASE(1024, 8, 1);
+	else if (cols <= 4096) TFHIP_LN_CASE(512, 8, 1);
+	else if (cols <= 8192) TFHIP_LN_CASE(512, 16, 1);
 	else TFHIP_LN_CASE(1024, 16, 1);
 #undef TFHIP_LN_CASE
 }
@@ -456,9 +470,10 @@ static int layer_norm_backward(const float* x, const float* dy, const float* wei
 	return rc;
 }
 
+template <int VEC>
 static int layer_norm_long_backward(const float* x, const float* dy, const float* weight, const float* mean, const float* rstd, float* dx, float* dweight, float* dbias, size_t rows, size_t cols) {
 	State& s = state();
-	const size_t segments = (cols + kLnSegment - 1) / kLnSegment, col_tiles = (cols + kLnThreads - 1) / kLnThreads;
+	const size_t segments = (cols + kLnSegment - 1) / kLnSegment, col_tiles = (cols + kLnThreads * VEC - 1) / (kLnThreads * VEC);
 	if (rows * segments > 0x7FFFFFFF) return fail(TFHIP_ERR_ARG, "layer norm of %zu x %zu is too large", rows, cols);
 	size_t slabs = (size_t)s.compute_units * 8 / col_tiles;
 	if (slabs > (rows + 15) / 16) slabs = (rows + 15) / 16;
@@ -471,21 +486,22 @@ static int layer_norm_long_backward(const float* x, const float* dy, const float
 	float2* stats = (float2*)base;
 	float* partial = (float*)(base + stats_bytes);
 	if (dweight || dbias) {  // before dx, which may overwrite x or dy
-		hipLaunchKernelGGL(layer_norm_dweight_kernel, dim3((unsigned)(col_tiles * slabs)), dim3(kLnThreads), 0, s.stream, x, dy, mean, rstd, partial, rows, cols, per, (unsigned)col_tiles);
+		hipLaunchKernelGGL(layer_norm_dweight_kernel<VEC>, dim3((unsigned)(col_tiles * slabs)), dim3(kLnThreads), 0, s.stream, x, dy, mean, rstd, partial, rows, cols, per, (unsigned)col_tiles);
 		TFHIP_CHECK_LAUNCH();
 		const int rc = launch_fold(partial, dweight, dbias, slabs, cols);
 		if (rc) return rc;
 	}
 	if (dx) {
 		const dim3 grid((unsigned)(rows * segments)), block(kLnThreads);
-		hipLaunchKernelGGL(layer_norm_segment_sums_kernel, grid, block, 0, s.stream, x, dy, weight, mean, rstd, stats, (int)cols, (int)segments);
+		hipLaunchKernelGGL(layer_norm_segment_sums_kernel<VEC>, grid, block, 0, s.stream, x, dy, weight, mean, rstd, stats, (int)cols, (int)segments);
 		TFHIP_CHECK_LAUNCH();
-		hipLaunchKernelGGL(layer_norm_segment_dx_kernel, grid, block, 0, s.stream, x, dy, weight, mean, rstd, dx, (const float2*)stats, (int)cols, (int)segments);
+		hipLaunchKernelGGL(layer_norm_segment_dx_kernel<VEC>, grid, block, 0, s.stream, x, dy, weight, mean, rstd, dx, (const float2*)stats, (int)cols, (int)segments);
 		TFHIP_CHECK_LAUNCH();
 	}
 	return TFHIP_OK;
 }
 
+template <int VEC>
 static int layer_norm_long_forward(const float* x, const float* weight, const float* bias, float* y, float* mean, float* rstd, size_t rows, size_t cols, float eps) {
 	State& s = state();
 	const size_t segments = (cols + kLnSegment - 1) / kLnSegment;
@@ -493,9 +509,9 @@ static int layer_norm_long_forward(const float* x, const float* weight, const fl
 	float2* stats = (float2*)scratch(rows * segments * sizeof(float2));
 	if (!stats) return TFHIP_ERR_HIP;
 	const dim3 grid((unsigned)(rows * segments)), block(kLnThreads);
-	hipLaunchKernelGGL(layer_norm_segment_kernel, grid, block, 0, s.stream, x, stats, (int)cols, (int)segments);
+	hipLaunchKernelGGL(layer_norm_segment_kernel<VEC>, grid, block, 0, s.stream, x, stats, (int)cols, (int)segments);
 	TFHIP_CHECK_LAUNCH();
-	hipLaunchKernelGGL(layer_norm_apply_kernel, grid, block, 0, s.stream, x, weight, bias, y, mean, rstd, (const float2*)stats, (int)cols, (int)segments, eps);
+	hipLaunchKernelGGL(layer_norm_apply_kernel<VEC>, grid, block, 0, s.stream, x, weight, bias, y, mean, rstd, (const float2*)stats, (int)cols, (int)segments, eps);
 	TFHIP_CHECK_LAUNCH();
 	return TFHIP_OK;
 }
@@ -541,9 +557,9 @@ extern "C" int tfhip_layer_norm_rows_f32(const float* x, const float* weight, co
 	if (rc) return rc;
 	TFHIP_REQUIRE_INIT();
 	TFHIP_HOLD_DEVICE();
-	if (cols > kLnMostInRegisters) return layer_norm_long_forward(x, weight, bias, y, mean, rstd, rows, cols, eps);
-	if (cols % 4 == 0 && aligned16(x, y, weight, bias)) return layer_norm_forward<4>(x, weight, bias, y, mean, rstd, rows, cols, eps);
-	return layer_norm_forward<1>(x, weight, bias, y, mean, rstd, rows, cols, eps);
+	const bool vec = cols % 4 == 0 && aligned16(x, y, weight, bias);
+	if (cols > kLnMostInRegisters) return (vec ? layer_norm_long_forward<4> : layer_norm_long_forward<1>)(x, weight, bias, y, mean, rstd, rows, cols, eps);
+	return (vec ? layer_norm_forward<4> : layer_norm_forward<1>)(x, weight, bias, y, mean, rstd, rows, cols, eps);
 }
 
 extern "C" int tfhip_layer_norm_rows_backward_f32(const float* x, const float* dy, const float* weight, const float* mean, const float* rstd, float* dx, float* dweight, float* dbias, size_t rows,
@@ -563,7 +579,7 @@ extern "C" int tfhip_layer_norm_rows_backward_f32(const float* x, const float* d
 		if (dbias && (rc = tfhip_fill_u32(dbias, 0u, cols))) return rc;
 		return TFHIP_OK;
 	}
-	if (cols > kLnMostInRegisters) return layer_norm_long_backward(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, cols);
-	if (cols % 4 == 0 && aligned16(x, dy, weight, dx)) return layer_norm_backward<4>(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, cols);
-	return layer_norm_backward<1>(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, cols);
+	const bool vec = cols % 4 == 0 && aligned16(x, dy, weight, dx);
+	if (cols > kLnMostInRegisters) return (vec ? layer_norm_long_backward<4> : layer_norm_long_backward<1>)(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, cols);
+	return (vec ? layer_norm_backward<4> : layer_norm_backward<1>)(x, dy, weight, mean, rstd, dx, dweight, dbias, rows, cols);
 }
