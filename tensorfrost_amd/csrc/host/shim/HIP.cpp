@@ -123,6 +123,11 @@ static void DispatchPrimitive(const HipKernelInfo* kernel, const TFDispatchInfo&
 		return ((TFHipBuffer*)t.buffer)->GetNative();
 	};
 	auto var = [&](size_t i) { return (size_t)info.variables[i]; };
+	auto real = [&](size_t i) {
+		float v;
+		memcpy(&v, &info.variables[i], sizeof(v));
+		return v;
+	};
 	int status;
 	if (p.rfind("sgemm_", 0) == 0) {
 		// sgemm_<nn|nt|tn>[_<bias|bias_relu|mask_positive>]
@@ -150,6 +155,21 @@ static void DispatchPrimitive(const HipKernelInfo* kernel, const TFDispatchInfo&
 		const int code = kind == "u32" ? TFHIP_KEY_U32 : kind == "i32" ? TFHIP_KEY_I32 : kind == "f32" ? TFHIP_KEY_F32 : -1;
 		if (code < 0) throw std::runtime_error("Unknown primitive " + p);
 		status = tfhip_radix_sort_kv(code, (const uint32_t*)buf(4), (const uint32_t*)buf(5), (uint32_t*)buf(0), (uint32_t*)buf(1), (uint32_t*)buf(2), (uint32_t*)buf(3), var(0));
+	} else if (p == "layer_norm_rows") {
+		status = tfhip_layer_norm_rows_f32((const float*)buf(3), (const float*)buf(4), (const float*)buf(5), (float*)buf(0), (float*)buf(1), (float*)buf(2), var(0), var(1), real(2));
+	} else if (p == "layer_norm_rows_backward") {
+		status = tfhip_layer_norm_rows_backward_f32((const float*)buf(3), (const float*)buf(4), (const float*)buf(5), (const float*)buf(6), (const float*)buf(7), (float*)buf(0), (float*)buf(1),
+		                                            (float*)buf(2), var(0), var(1));
+	} else if (p == "embedding_rows") {
+		status = tfhip_embedding_rows_f32((const int32_t*)buf(1), (const float*)buf(2), (float*)buf(0), var(0), var(1), var(2), real(3));
+	} else if (p == "embedding_rows_backward") {
+		status = tfhip_embedding_rows_backward_f32((const int32_t*)buf(1), (const float*)buf(2), (float*)buf(0), var(0), var(1), var(2), real(3));
+	} else if (p == "newton_schulz") {
+		const int steps = (int)var(3);
+		std::vector<float> coefficients;
+		for (int k = 0; k < steps && k < 64; k++)
+			for (size_t i = 0; i < 3; i++) coefficients.push_back(real(5 + i));
+		status = tfhip_newton_schulz_f32((const float*)buf(1), (float*)buf(0), var(0), var(1), var(2), steps, coefficients.data(), real(4));
 	} else {
 		throw std::runtime_error("Unknown primitive " + p);
 	}

@@ -201,7 +201,10 @@ class Program {
 	// sgemm_nn|sgemm_nt|sgemm_tn {C | A, B} (M, N, K); with a fused tail, sgemm_<layout>_bias|_bias_relu {C | A, B, bias[N]}
 	// and sgemm_<layout>_mask_positive {C | A, B, mask[M,N]}; reduce_rows_<op>|reduce_cols_<op> {out | x} (rows, cols);
 	// softmax_rows {y | x} (rows, cols); scan_u32|scan_i32|scan_f32 {out | x} (n);
-	// radix_sort_kv_u32|_i32|_f32 {keys_out, vals_out, keys_tmp, vals_tmp | keys_in, vals_in} (n).
+	// radix_sort_kv_u32|_i32|_f32 {keys_out, vals_out, keys_tmp, vals_tmp | keys_in, vals_in} (n);
+	// layer_norm_rows {y, mean, rstd | x, weight, bias} (rows, cols, eps); layer_norm_rows_backward {dx, dweight, dbias | x,
+	// dy, weight, mean, rstd} (rows, cols); embedding_rows {out | tokens, table} and embedding_rows_backward {dtable | tokens, dy}
+	// (n, vocab, cols, scale); newton_schulz {out | g} (batch, rows, cols, steps, eps, a, b, c); real scalars as their bits.
 	Kernel* AddPrimitive(const std::string& name, size_t n_tensors, size_t n_variables);
 };
 
