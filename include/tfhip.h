@@ -249,7 +249,8 @@ int tfhip_sgemm_batched(int layout, const float* A, const float* B, float* C, si
  * the mean and norm reductions, loads with computed indices and atomic adds (Compiler/Implementations.cpp:243-303,
  * 451-488), and its optimisers end at the element-wise update (Python/TensorFrost/optimizers.py:104-167). All matrices
  * are dense row-major fp32; every sum is held in fp32 or wider, in an order that does not change from run to run.
- * Several host threads may make these calls at once: the launches of one call stay together on the library's stream.
+ * Several host threads may call these and the primitives above at once: the launches of one call stay together on the
+ * library's stream. The library's device is made current for the length of a call.
  * They may be recorded into a graph (run the same work once before, so that the scratch buffer has its size). */
 
 /* y[r,c] = (x[r,c] - mean[r]) * rstd[r] * weight[c] + bias[c], mean[r] = mean_c x[r,:], rstd[r] = 1 / sqrt(mean_c (x[r,:] -

@@ -455,12 +455,14 @@ extern "C" {
 int tfhip_radix_sort_kv(int key_kind, const uint32_t* keys_in, const uint32_t* vals_in, uint32_t* keys_out, uint32_t* vals_out,
                         uint32_t* keys_tmp, uint32_t* vals_tmp, size_t n) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	return radix_sort_impl(key_kind, keys_in, vals_in, keys_out, vals_out, keys_tmp, vals_tmp, n);
 }
 
 int tfhip_radix_sort_kv_u32(const uint32_t* keys_in, const uint32_t* vals_in, uint32_t* keys_out, uint32_t* vals_out,
                             uint32_t* keys_tmp, uint32_t* vals_tmp, size_t n) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	return radix_sort_impl(kKeyU32, keys_in, vals_in, keys_out, vals_out, keys_tmp, vals_tmp, n);
 }
 

@@ -818,6 +818,7 @@ extern "C" {
 
 int tfhip_reduce_rows_f32(int op, const float* x, float* out, size_t rows, size_t cols) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	int rc = check_args(x, out, rows, cols);
 	if (rc) return rc;
 	switch (op) {
@@ -830,6 +831,7 @@ int tfhip_reduce_rows_f32(int op, const float* x, float* out, size_t rows, size_
 
 int tfhip_reduce_cols_slabs_f32(int op, const float* x, float* out, size_t rows, size_t cols, size_t rows_per_slab) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	int rc = check_args(x, out, rows, cols);
 	if (rc) return rc;
 	if (rows_per_slab == 0) return fail(TFHIP_ERR_ARG, "rows_per_slab must be positive");
@@ -843,6 +845,7 @@ int tfhip_reduce_cols_slabs_f32(int op, const float* x, float* out, size_t rows,
 
 int tfhip_reduce_cols_f32(int op, const float* x, float* out, size_t rows, size_t cols) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	int rc = check_args(x, out, rows, cols);
 	if (rc) return rc;
 	switch (op) {

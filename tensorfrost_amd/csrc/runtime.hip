@@ -833,6 +833,7 @@ int tfhip_scratch_info(size_t* bytes, size_t* retired_buffers, size_t* live_grap
 
 int tfhip_scratch_reserve(size_t bytes) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	return scratch(bytes) ? TFHIP_OK : TFHIP_ERR_HIP;
 }
 

@@ -765,6 +765,7 @@ extern "C" {
 // the other; many rows get one or four waves each.
 int tfhip_scan_inclusive_rows_u32(const uint32_t* in, uint32_t* out, size_t rows, size_t cols) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (rows == 0 || cols == 0) return TFHIP_OK;
 	if (!in || !out) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_scan_inclusive_rows_u32");
 	if (rows <= 4 && cols >= ((size_t)1 << 22)) {
@@ -779,6 +780,7 @@ int tfhip_scan_inclusive_rows_u32(const uint32_t* in, uint32_t* out, size_t rows
 
 int tfhip_scan_inclusive_rows_f32(const float* in, float* out, size_t rows, size_t cols) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (rows == 0 || cols == 0) return TFHIP_OK;
 	if (!in || !out) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_scan_inclusive_rows_f32");
 	if (rows <= 4 && cols >= ((size_t)1 << 22)) {
@@ -793,6 +795,7 @@ int tfhip_scan_inclusive_rows_f32(const float* in, float* out, size_t rows, size
 
 int tfhip_scan_inclusive_cols_u32(const uint32_t* in, uint32_t* out, size_t batch, size_t rows, size_t cols) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (batch == 0 || rows == 0 || cols == 0) return TFHIP_OK;
 	if (!in || !out) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_scan_inclusive_cols_u32");
 	return scan_cols<uint32_t>(in, out, batch, rows, cols);
@@ -800,6 +803,7 @@ int tfhip_scan_inclusive_cols_u32(const uint32_t* in, uint32_t* out, size_t batc
 
 int tfhip_scan_inclusive_cols_f32(const float* in, float* out, size_t batch, size_t rows, size_t cols) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (batch == 0 || rows == 0 || cols == 0) return TFHIP_OK;
 	if (!in || !out) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_scan_inclusive_cols_f32");
 	return scan_cols<float>(in, out, batch, rows, cols);
@@ -807,6 +811,7 @@ int tfhip_scan_inclusive_cols_f32(const float* in, float* out, size_t batch, siz
 
 int tfhip_scan_inclusive_u32(const uint32_t* in, uint32_t* out, size_t n) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (n == 0) return TFHIP_OK;
 	if (!in || !out) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_scan_inclusive_u32");
 	State& s = state();
@@ -829,6 +834,7 @@ int tfhip_scan_inclusive_u32(const uint32_t* in, uint32_t* out, size_t n) {
 // tile and exits; nothing waits without bound.
 int tfhip_test_scan_u32_first_tile_absent(const uint32_t* in, uint32_t* out, size_t n, uint32_t spin_limit) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (!in || !out) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_test_scan_u32_first_tile_absent");
 	State& s = state();
 	const size_t tiles = (n + LookbackCfg::tile - 1) / LookbackCfg::tile;
@@ -854,6 +860,7 @@ int tfhip_scan_inclusive_i32(const int32_t* in, int32_t* out, size_t n) {
 
 int tfhip_scan_inclusive_u32_static(const uint32_t* in, uint32_t* out, size_t n) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (n == 0) return TFHIP_OK;
 	if (!in || !out) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_scan_inclusive_u32_static");
 	if (n > kStaticScanMaxElements)
@@ -876,6 +883,7 @@ int tfhip_scan_inclusive_u32_static(const uint32_t* in, uint32_t* out, size_t n)
 
 int tfhip_scan_inclusive_f32(const float* in, float* out, size_t n) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (n == 0) return TFHIP_OK;
 	if (!in || !out) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_scan_inclusive_f32");
 	return scan_reduce_then_scan<float>(in, out, n);

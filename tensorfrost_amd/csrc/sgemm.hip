@@ -1846,24 +1846,29 @@ extern "C" {
 
 int tfhip_sgemm_nn(const float* A, const float* B, float* C, size_t M, size_t N, size_t K) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	return sgemm_impl(kNN, A, B, C, M, N, K);
 }
 int tfhip_sgemm_nt(const float* A, const float* B, float* C, size_t M, size_t N, size_t K) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	return sgemm_impl(kNT, A, B, C, M, N, K);
 }
 int tfhip_sgemm_tn(const float* A, const float* B, float* C, size_t M, size_t N, size_t K) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	return sgemm_impl(kTN, A, B, C, M, N, K);
 }
 int tfhip_sgemm_tn_colsum(const float* A, const float* B, float* C, float* colsum_b, size_t M, size_t N, size_t K) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (!colsum_b) return fail(TFHIP_ERR_ARG, "null pointer passed to tfhip_sgemm_tn_colsum");
 	return sgemm_impl(kTN, A, B, C, M, N, K, TFHIP_EPILOGUE_NONE, nullptr, 1, 0, 0, 0, colsum_b);
 }
 int tfhip_sgemm_batched(int layout, const float* A, const float* B, float* C, size_t M, size_t N, size_t K, size_t batch, size_t stride_a, size_t stride_b,
                         size_t stride_c) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (layout != TFHIP_GEMM_NN && layout != TFHIP_GEMM_NT && layout != TFHIP_GEMM_TN) return fail(TFHIP_ERR_ARG, "unknown sgemm layout %d", layout);
 	if (batch == 0) return fail(TFHIP_ERR_ARG, "sgemm over an empty batch");
 	if (batch > 1 && stride_c < M * N) return fail(TFHIP_ERR_ARG, "the results of a batch overlap (stride %zu for %zu x %zu)", stride_c, M, N);
@@ -1872,6 +1877,7 @@ int tfhip_sgemm_batched(int layout, const float* A, const float* B, float* C, si
 
 int tfhip_sgemm_fused(int layout, const float* A, const float* B, float* C, size_t M, size_t N, size_t K, int epilogue, const float* aux) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (layout != TFHIP_GEMM_NN && layout != TFHIP_GEMM_NT && layout != TFHIP_GEMM_TN) return fail(TFHIP_ERR_ARG, "unknown sgemm layout %d", layout);
 	return sgemm_impl(layout, A, B, C, M, N, K, epilogue, aux);
 }

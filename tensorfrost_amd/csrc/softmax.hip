@@ -359,6 +359,7 @@ using namespace tfhip;
 
 static int softmax_rows(const float* x, float* y, size_t rows, size_t cols, float* row_max, float* row_sum, bool log_form) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (!x || (!y && !row_max)) return fail(TFHIP_ERR_ARG, "null pointer passed to the row softmax");
 	if (rows == 0 || cols == 0) return fail(TFHIP_ERR_ARG, "softmax over an empty matrix (%zu x %zu)", rows, cols);
 	State& s = state();
