@@ -311,19 +311,20 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const uint32_t* __re
 		return;
 	}
 	const int lane = threadIdx.x & 63;
-	const uint32_t v0 = ((blockIdx.x - sum_groups) * 4 + (threadIdx.x >> 6)) * kZeroRows;
-	if (v0 >= vocab) return;
-	bool idle = false;
-	if (lane < kZeroRows && v0 + lane < vocab) {
-		const uint32_t at = first_at_least(keys, n, v0 + lane);
-		idle = at >= n || keys[at] != v0 + lane;
-	}
-	uint64_t rows = __ballot(idle);
-	while (rows) {
-		const int r = __builtin_ctzll(rows);
-		rows &= rows - 1;
-		float* to = dtable + (size_t)(v0 + r) * cols;
-		for (size_t c = (size_t)lane * VEC; c < cols; c += 64 * VEC) __builtin_nontemporal_store(Vec(0.0f), reinterpret_cast<Vec*>(to + c));
+	const uint64_t step = (uint64_t)(gridDim.x - sum_groups) * 4 * kZeroRows;
+	for (uint64_t v0 = ((uint64_t)(blockIdx.x - sum_groups) * 4 + (threadIdx.x >> 6)) * kZeroRows; v0 < vocab; v0 += step) {
+		bool idle = false;
+		if (lane < kZeroRows && v0 + lane < vocab) {
+			const uint32_t v = (uint32_t)v0 + lane, at = first_at_least(keys, n, v);
+			idle = at >= n || keys[at] != v;
+		}
+		uint64_t rows = __ballot(idle);
+		while (rows) {
+			const int r = __builtin_ctzll(rows);
+			rows &= rows - 1;
+			float* to = dtable + (size_t)(v0 + r) * cols;
+			for (size_t c = (size_t)lane * VEC; c < cols; c += 64 * VEC) __builtin_nontemporal_store(Vec(0.0f), reinterpret_cast<Vec*>(to + c));
+		}
 	}
 }
 
@@ -385,8 +386,10 @@ static int embedding_sums(const uint32_t* keys, const uint32_t* order, const flo
 	State& s = state();
 	const uint32_t segments = (n + segment - 1) / segment;
 	const size_t col_steps = (cols + (size_t)lanes * VEC - 1) / ((size_t)lanes * VEC);
-	const size_t sum_groups = ((size_t)segments * col_steps * lanes + 255) / 256, zero_groups = ((size_t)vocab + kZeroRows * 4 - 1) / (kZeroRows * 4);
-	if (sum_groups + zero_groups > 0x7FFFFFFF) return fail(TFHIP_ERR_ARG, "embedding gradient of %u tokens with %zu columns is too large", n, cols);
+	const size_t sum_groups = ((size_t)segments * col_steps * lanes + 255) / 256;
+	size_t zero_groups = ((size_t)vocab + kZeroRows * 4 - 1) / (kZeroRows * 4);
+	if (zero_groups > 1 << 20) zero_groups = 1 << 20;
+	if (sum_groups + zero_groups > 0xFFFFFF) return fail(TFHIP_ERR_ARG, "embedding gradient of %u tokens with %zu columns is too large", n, cols);
 	hipLaunchKernelGGL(embedding_sum_kernel<VEC>, dim3((unsigned)(sum_groups + zero_groups)), dim3(256), 0, s.stream, keys, order, dy, dtable, partial, n, vocab, cols, scale, segment, segments,
 	                   lanes, (uint32_t)col_steps, (uint32_t)sum_groups);
 	TFHIP_CHECK_LAUNCH();
@@ -447,7 +450,8 @@ extern "C" int tfhip_embedding_rows_backward_f32(const int32_t* tokens, const fl
 	while (digits < 4 && vocab >> (8 * digits)) digits++;
 	// Rows a wave adds up one after the other: few rows need shorter chains, more of them at once (500 x 250: sums and
 	// joins 9.6 us with 16, 11.3 with 32, 16.5 with 64), many rows fewer parts to join (65536 x 1024: 93, 89 and 88.5 us).
-	const uint32_t segment = n * cols >= (size_t)1 << 22 ? 32 : 16;
+	uint32_t segment = n * cols >= (size_t)1 << 22 ? 32 : 16;
+	while (n / segment >= (size_t)1 << 22) segment *= 2;  // a launch has fewer than 2^32 threads
 	const size_t segments = (n + segment - 1) / segment;
 	// [the library sort's own words][keys, order sorted][keys, order between passes, and before them][counts][parts of the runs]
 	const size_t words = (n + 63) & ~size_t(63);

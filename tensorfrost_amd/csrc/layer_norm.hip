@@ -377,26 +377,31 @@ constexpr int kFoldWaves = 16;
 __global__ __launch_bounds__(kFoldWaves * 64) void layer_norm_fold_kernel(const float* __restrict__ partial, float* __restrict__ dweight, float* __restrict__ dbias, size_t parts, size_t cols) {
 	__shared__ float red[kFoldWaves][64];
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-	const size_t c = (size_t)blockIdx.x * 64 + lane, width = 2 * cols;
-	float sum = 0.0f;
-	if (c < width) {
-		size_t k = wave;
-		for (; k + 7 * kFoldWaves < parts; k += 8 * kFoldWaves) {
-			float t[8];
+	const size_t width = 2 * cols;
+	for (size_t c0 = (size_t)blockIdx.x * 64; c0 < width; c0 += (size_t)gridDim.x * 64) {
+		const size_t c = c0 + lane;
+		float sum = 0.0f;
+		if (c < width) {
+			size_t k = wave;
+			for (; k + 7 * kFoldWaves < parts; k += 8 * kFoldWaves) {
+				float t[8];
 #pragma unroll
-			for (int u = 0; u < 8; u++) t[u] = partial[(k + u * kFoldWaves) * width + c];
+				for (int u = 0; u < 8; u++) t[u] = partial[(k + u * kFoldWaves) * width + c];
 #pragma unroll
-			for (int u = 0; u < 8; u++) sum += t[u];
+				for (int u = 0; u < 8; u++) sum += t[u];
+			}
+			for (; k < parts; k += kFoldWaves) sum += partial[k * width + c];
 		}
-		for (; k < parts; k += kFoldWaves) sum += partial[k * width + c];
-	}
-	red[wave][lane] = sum;
-	__syncthreads();
-	if (wave != 0 || c >= width) return;
+		red[wave][lane] = sum;
+		__syncthreads();
+		if (wave == 0 && c < width) {
 #pragma unroll
-	for (int w = 1; w < kFoldWaves; w++) sum += red[w][lane];
-	float* to = c < cols ? dweight : dbias;
-	if (to) to[c < cols ? c : c - cols] = sum;
+			for (int w = 1; w < kFoldWaves; w++) sum += red[w][lane];
+			float* to = c < cols ? dweight : dbias;
+			if (to) to[c < cols ? c : c - cols] = sum;
+		}
+		__syncthreads();
+	}
 }
 
 // ---- which kernel ------------------------------------------------------------------------------------
@@ -430,15 +435,21 @@ static int layer_norm_forward(const float* x, const float* weight, const float* 
 	State& s = state();
 	with_row_group<VEC>(cols, [&](auto group, auto e, auto vec, auto r) {
 		constexpr int kGroup = decltype(group)::value, kThreads = kGroup > 256 ? kGroup : 256, kRows = kThreads / kGroup * decltype(r)::value;
-		hipLaunchKernelGGL((layer_norm_kernel<kGroup, decltype(e)::value, decltype(vec)::value, decltype(r)::value>), dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(kThreads), 0, s.stream, x,
-		                   weight, bias, y, mean, rstd, rows, (int)cols, eps);
+		// a launch has fewer than 2^32 threads
+		constexpr size_t kMost = ((size_t)1 << 31) / kThreads * kRows;
+		for (size_t first = 0; first < rows; first += kMost) {
+			const size_t count = rows - first < kMost ? rows - first : kMost;
+			hipLaunchKernelGGL((layer_norm_kernel<kGroup, decltype(e)::value, decltype(vec)::value, decltype(r)::value>), dim3((unsigned)((count + kRows - 1) / kRows)), dim3(kThreads), 0, s.stream,
+			                   x + first * cols, weight, bias, y + first * cols, mean ? mean + first : nullptr, rstd ? rstd + first : nullptr, count, (int)cols, eps);
+		}
 	});
 	TFHIP_CHECK_LAUNCH();
 	return TFHIP_OK;
 }
 
 static int launch_fold(const float* partial, float* dweight, float* dbias, size_t parts, size_t cols) {
-	hipLaunchKernelGGL(layer_norm_fold_kernel, dim3((unsigned)((2 * cols + 63) / 64)), dim3(kFoldWaves * 64), 0, state().stream, partial, dweight, dbias, parts, cols);
+	const size_t groups = (2 * cols + 63) / 64;
+	hipLaunchKernelGGL(layer_norm_fold_kernel, dim3((unsigned)(groups < 65536 ? groups : 65536)), dim3(kFoldWaves * 64), 0, state().stream, partial, dweight, dbias, parts, cols);
 	TFHIP_CHECK_LAUNCH();
 	return TFHIP_OK;
 }
@@ -474,7 +485,7 @@ template <int VEC>
 static int layer_norm_long_backward(const float* x, const float* dy, const float* weight, const float* mean, const float* rstd, float* dx, float* dweight, float* dbias, size_t rows, size_t cols) {
 	State& s = state();
 	const size_t segments = (cols + kLnSegment - 1) / kLnSegment, col_tiles = (cols + kLnThreads * VEC - 1) / (kLnThreads * VEC);
-	if (rows * segments > 0x7FFFFFFF) return fail(TFHIP_ERR_ARG, "layer norm of %zu x %zu is too large", rows, cols);
+	if (rows * segments > 0xFFFFFF) return fail(TFHIP_ERR_ARG, "layer norm of %zu x %zu is too large", rows, cols);
 	size_t slabs = (size_t)s.compute_units * 8 / col_tiles;
 	if (slabs > (rows + 15) / 16) slabs = (rows + 15) / 16;
 	if (slabs < 1) slabs = 1;
@@ -505,7 +516,7 @@ template <int VEC>
 static int layer_norm_long_forward(const float* x, const float* weight, const float* bias, float* y, float* mean, float* rstd, size_t rows, size_t cols, float eps) {
 	State& s = state();
 	const size_t segments = (cols + kLnSegment - 1) / kLnSegment;
-	if (rows * segments > 0x7FFFFFFF) return fail(TFHIP_ERR_ARG, "layer norm of %zu x %zu is too large", rows, cols);
+	if (rows * segments > 0xFFFFFF) return fail(TFHIP_ERR_ARG, "layer norm of %zu x %zu is too large", rows, cols);
 	float2* stats = (float2*)scratch(rows * segments * sizeof(float2));
 	if (!stats) return TFHIP_ERR_HIP;
 	const dim3 grid((unsigned)(rows * segments)), block(kLnThreads);

@@ -524,8 +524,8 @@ static double largest_square(double b, double c, double top) {
 
 // The power of two that brings values of at most `bound` to at most 2^15.
 static double scale_for(double bound) {
-	if (!(bound > 1e-18)) bound = 1e-18;
-	if (!(bound < 1e18)) bound = 1e18;
+	if (!(bound > 1e-30)) bound = 1e-30;
+	if (!(bound < 1e37)) bound = 1e37;
 	int e;
 	frexp(bound, &e);  // bound <= 2^e
 	return ldexp(1.0, 15 - e);

@@ -151,3 +151,30 @@ def test_offsets_past_32_bits(rt):
     for v in (1, (1 << 19) - 1, (1 << 19) + 1, vocab - 2):
         assert not table.numpy(np.float32, (cols,), offset_words=v * cols).any(), v
     table.free()
+
+
+def test_many_rows_of_one_column(rt):
+    """A table of 2^29 + 7 rows, more than a launch has waves for: every row is written."""
+    vocab = (1 << 29) + 7
+    d = rt.DeviceBuffer(vocab)
+    d.fill(0x7FC00000)
+    t = np.array([0, vocab - 1, 1 << 28, vocab - 1, -1], np.int32)
+    rt.embedding_rows_backward(rt.DeviceBuffer.from_numpy(t), rt.DeviceBuffer.from_numpy(np.array([1, 2, 3, 4, 5], np.float32)), d, 5, vocab, 1)
+    got = d.numpy()
+    assert got[0] == 1 and got[vocab - 1] == 6 and got[1 << 28] == 3
+    got[[0, vocab - 1, 1 << 28]] = 0
+    assert not got.any()
+    d.free()
+
+
+def test_many_positions_of_one_token(rt):
+    """2^28 positions, more parts than a launch has groups of eight waves for. Sums of ones over 64 and more positions are multiples
+    of 64 below 2^29: exact."""
+    n = 1 << 28
+    t, dy, d = rt.DeviceBuffer(n), rt.DeviceBuffer(n), rt.DeviceBuffer(10)
+    t.fill(7)
+    dy.fill(0x3F800000)
+    rt.embedding_rows_backward(t, dy, d, n, 10, 1, scale=0.5)
+    assert np.array_equal(d.numpy(), np.where(np.arange(10) == 7, n / 2, 0).astype(np.float32))
+    for b in (t, dy):
+        b.free()

@@ -229,3 +229,40 @@ def test_backward_against_differences(rt):
             down, step_down = loss(x, w, b), float(array[at])
             array[at] = keep
             assert abs((up - down) / (step_up - step_down) - grad[at]) < 2e-2
+
+
+def test_a_row_of_many_columns(rt):
+    """140 000 001 columns: more than a launch of one group per 64 columns of the two gradients covers. x = +-1 in turn and one 0: mean 0
+    (whole numbers below 2^24 in every partial sum of 8192), variance 1 up to 1e-8 and the rounding of sums."""
+    cols = 140_000_001
+    x = np.ones(cols, np.float32)
+    x[1::2] = -1
+    x[-1] = 0
+    dy = (np.arange(cols) % 5 - 2).astype(np.float32)
+    xb, dyb = rt.DeviceBuffer.from_numpy(x), rt.DeviceBuffer.from_numpy(dy)
+    y, mean, rstd, dw, db = rt.DeviceBuffer(cols), rt.DeviceBuffer(1), rt.DeviceBuffer(1), rt.DeviceBuffer(cols), rt.DeviceBuffer(cols)
+    rt.layer_norm_rows(xb, None, None, y, 1, cols, eps=0.0, mean=mean, rstd=rstd)
+    assert mean.numpy()[0] == 0 and abs(rstd.numpy()[0] - 1) < 1e-5
+    s = rstd.numpy()[0]
+    assert np.array_equal(y.numpy(), x * s)
+    rt.layer_norm_rows_backward(xb, dyb, None, mean, rstd, 1, cols, dweight=dw, dbias=db)
+    assert np.array_equal(db.numpy(), dy) and np.array_equal(dw.numpy(), dy * (x * s))
+    for b in (xb, dyb, y, dw, db):
+        b.free()
+
+
+def test_many_rows_of_one_column_in_place(rt):
+    """2^30 + 3 rows of one element: each is its own mean, so y = bias everywhere; two launches."""
+    rows = (1 << 30) + 3
+    x, mean = rt.DeviceBuffer(rows), rt.DeviceBuffer(rows)
+    x.fill(0x40400000)
+    rt.layer_norm_rows(x, None, rt.DeviceBuffer.from_numpy(np.array([0.25], np.float32)), x, rows, 1, mean=mean)
+    for b, want in ((x, 0.25), (mean, 3.0)):
+        for at in (0, rows // 2, (1 << 29) - 2, rows - 5):
+            assert (b.numpy(np.float32, (5,), offset_words=at) == want).all()
+        out = rt.DeviceBuffer(1)
+        rt.reduce_rows("min", b, out, 1, rows)
+        assert out.numpy()[0] == want
+        rt.reduce_rows("max", b, out, 1, rows)
+        assert out.numpy()[0] == want
+        b.free()
