@@ -493,6 +493,207 @@ __global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const 
 	finish_tile<KIND>(g, v, addend, tp * T, tq * T, tp == tq, reinterpret_cast<uint32_t*>(lds));
 }
 
+// ---- small matrices: every step in one group ----------------------------------------------------------
+
+// A matrix of at most 64 x 256 (the first and last layers of a small network) stays in the group memory of one compute unit
+// from its norm to its last product: X, its transpose and A (then B in its place) in split form, 2 * 64 * NP * 4 B + 16 KiB. One
+// launch instead of seventeen, which cost 4 to 5 us each whatever they compute.
+// The results are written turned (four rows of a lane are four neighbours: 8-byte writes), so X comes from the product
+// X^T B and X^T from B X; the second product costs less than the 2-byte writes of the other orientation.
+constexpr int kSmallRows = 64, kSmallThreads = 512;
+constexpr size_t kSmallCols = 256;
+
+struct NsSmallArgs {
+	const float* g;
+	float* out;
+	int m, n;  // rows and columns of X, m <= n
+	bool transposed;
+	float eps, scale;
+	int steps;
+	struct {
+		float gram, poly, poly_a, update, update_x;  // factors of A, A^2, A in B, B X, X
+	} step[64];
+};
+
+// Where piece c (16 bytes: 8 hi or, from c = 4 on, 8 lo) of block kb of a row lies. The sixteen pieces of two blocks are
+// exchanged by the row, so that the lanes that read one piece of 16 rows meet different banks.
+__device__ __forceinline__ int small_at(int row, int row_bytes, int kb, int c) { return row * row_bytes + (kb >> 1) * 256 + ((((kb & 1) * 8 + c) ^ (row & 15)) << 4); }
+
+template <int NP>
+__global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallArgs a) {
+	constexpr int kX = 0, kXt = kSmallRows * NP * 4, kA = 2 * kXt;  // byte offsets
+	constexpr int kRowX = NP * 4, kRowM = kSmallRows * 4;           // bytes of a row of X; of X^T and A
+	__shared__ __attribute__((aligned(256))) char lds[kA + kSmallRows * kSmallRows * 4];
+	__shared__ double red[kSmallThreads / 64];
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+	const int m = a.m, n = a.n;
+	const float* g = a.g + (size_t)blockIdx.x * m * n;
+
+	// two rows by two columns of X per thread and turn
+	constexpr int kTurns = kSmallRows * NP / 4 / kSmallThreads;
+	float v[kTurns][4];
+	double sum = 0.0;
+#pragma unroll
+	for (int t = 0; t < kTurns; t++) {
+		const int at = t * kSmallThreads + tid, r0 = at / (NP / 2) * 2, c0 = at % (NP / 2) * 2;
+#pragma unroll
+		for (int k = 0; k < 4; k++) {
+			const int r = r0 + (k >> 1), c = c0 + (k & 1);
+			v[t][k] = r < m && c < n ? (a.transposed ? g[(size_t)c * m + r] : g[(size_t)r * n + c]) : 0.0f;
+			sum += (double)v[t][k] * (double)v[t][k];
+		}
+	}
+	sum = wave_reduce(sum, [](double x, double y) { return x + y; });
+	if (lane == 0) red[wave] = sum;
+	__syncthreads();
+	sum = 0.0;
+#pragma unroll
+	for (int w = 0; w < kSmallThreads / 64; w++) sum += red[w];
+	const double norm = sqrt(sum) + (double)a.eps;
+	const double factor = !isfinite(norm) ? (double)nanf("") : norm > 0.0 ? (double)a.scale / norm : 0.0;
+#pragma unroll
+	for (int t = 0; t < kTurns; t++) {
+		const int at = t * kSmallThreads + tid, r0 = at / (NP / 2) * 2, c0 = at % (NP / 2) * 2;
+		uint32_t p[4];
+#pragma unroll
+		for (int k = 0; k < 4; k++) p[k] = split_pair((float)((double)v[t][k] * factor));
+#pragma unroll
+		for (int k = 0; k < 2; k++) {
+			// row r0 + k of X, columns c0 and c0 + 1; row c0 + k of X^T, columns r0 and r0 + 1
+			const uint32_t x0 = p[2 * k], x1 = p[2 * k + 1], t0 = p[k], t1 = p[2 + k];
+			char* to = lds + kX + (c0 & 7) * 2;
+			*reinterpret_cast<uint32_t*>(to + small_at(r0 + k, kRowX, c0 >> 5, (c0 & 31) >> 3)) = (x0 & 0xFFFFu) | (x1 << 16);
+			*reinterpret_cast<uint32_t*>(to + small_at(r0 + k, kRowX, c0 >> 5, ((c0 & 31) >> 3) + 4)) = (x0 >> 16) | (x1 & 0xFFFF0000u);
+			to = lds + kXt + (r0 & 7) * 2;
+			*reinterpret_cast<uint32_t*>(to + small_at(c0 + k, kRowM, r0 >> 5, (r0 & 31) >> 3)) = (t0 & 0xFFFFu) | (t1 << 16);
+			*reinterpret_cast<uint32_t*>(to + small_at(c0 + k, kRowM, r0 >> 5, ((r0 & 31) >> 3) + 4)) = (t0 >> 16) | (t1 & 0xFFFF0000u);
+		}
+	}
+	__syncthreads();
+
+	// A lane's row of a tile is lane % 32 (tiles begin at multiples of 32), so what small_at exchanges by is the lane's own: the
+	// address of a piece is a lane's part, one exclusive or with a constant, and an offset that the wave shares.
+	const int lane_x = (lane & 31) * kRowX, lane_m = (lane & 31) * kRowM, read_at = ((lane & 15) ^ h) << 4, turned_at = (lane & 15) << 4;
+	// the 32 x 32 tile of rows p0.. of P times rows q0.. of Q over the blocks [kb0, kb1): low products and high ones apart
+	auto product = [&](floatx16& r, int P, int p_bytes, int p0, int Q, int q_bytes, int q0, int kb0, int kb1) {
+		floatx16 low, high;
+#pragma unroll
+		for (int i = 0; i < 16; i++) low[i] = high[i] = 0.0f;
+		const char* p = lds + P + p0 * p_bytes + (p_bytes == kRowX ? lane_x : lane_m);
+		const char* q = lds + Q + q0 * q_bytes + (q_bytes == kRowX ? lane_x : lane_m);
+#pragma unroll 2
+		for (int kb = kb0; kb < kb1; kb++) {
+			const int at = (kb >> 1) * 256, turn = read_at ^ ((kb & 1) << 7);
+#pragma unroll
+			for (int half = 0; half < 2; half++) {
+				const int hi = at + (turn ^ (half << 5)), lo = at + (turn ^ (half << 5) ^ 64);
+				const half8 p_hi = *reinterpret_cast<const half8*>(p + hi), p_lo = *reinterpret_cast<const half8*>(p + lo);
+				const half8 q_hi = *reinterpret_cast<const half8*>(q + hi), q_lo = *reinterpret_cast<const half8*>(q + lo);
+				low = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_lo, q_hi, low, 0, 0, 0);
+				high = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi, q_hi, high, 0, 0, 0);
+				low = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi, q_lo, low, 0, 0, 0);
+			}
+		}
+#pragma unroll
+		for (int i = 0; i < 16; i++) r[i] = low[i] + high[i];
+		__builtin_amdgcn_sched_barrier(0);  // one product at a time: four interleaved ones do not fit the registers
+	};
+	// r = alpha r + beta D, D turned: D[q0 + lane's column][p0 + rows]
+	auto add = [&](floatx16& r, float alpha, float beta, int D, int d_bytes, int p0, int q0) {
+		const char* d = lds + D + q0 * d_bytes + (d_bytes == kRowX ? lane_x : lane_m) + (p0 >> 6) * 256 + 8 * h;
+		const int turn = turned_at ^ (((p0 >> 5) & 1) << 7);
+#pragma unroll
+		for (int q = 0; q < 4; q++) {
+			const half4 hi = *reinterpret_cast<const half4*>(d + (turn ^ (q << 4))), lo = *reinterpret_cast<const half4*>(d + (turn ^ (q << 4) ^ 64));
+#pragma unroll
+			for (int i = 0; i < 4; i++) r[4 * q + i] = alpha * r[4 * q + i] + beta * ((float)hi[i] + (float)lo[i]);
+		}
+	};
+	auto store = [&](const floatx16& r, int D, int d_bytes, int p0, int q0) {
+		char* d = lds + D + q0 * d_bytes + (d_bytes == kRowX ? lane_x : lane_m) + (p0 >> 6) * 256 + 8 * h;
+		const int turn = turned_at ^ (((p0 >> 5) & 1) << 7);
+#pragma unroll
+		for (int q = 0; q < 4; q++) {
+			uint32_t s[4];
+#pragma unroll
+			for (int i = 0; i < 4; i++) s[i] = split_pair(r[4 * q + i]);
+			*reinterpret_cast<uint2*>(d + (turn ^ (q << 4))) = make_uint2((s[0] & 0xFFFFu) | (s[1] << 16), (s[2] & 0xFFFFu) | (s[3] << 16));
+			*reinterpret_cast<uint2*>(d + (turn ^ (q << 4) ^ 64)) = make_uint2((s[0] >> 16) | (s[1] & 0xFFFF0000u), (s[2] >> 16) | (s[3] & 0xFFFF0000u));
+		}
+	};
+
+	const int tile = wave & 3, ti = (tile >> 1) * 32, tj = (tile & 1) * 32;
+	constexpr int kBlocks = NP / 32;                 // of a row of X
+	constexpr int kShare = NP / 64;                  // products of X and of X^T per wave: 2 * 2 * kBlocks among eight
+	for (int k = 0; k < a.steps; k++) {
+		// A: four tiles, two waves each with half of the columns; the second halves pass through A's own place
+		floatx16 r;
+		product(r, kX, kRowX, ti, kX, kRowX, tj, wave < 4 ? 0 : kBlocks / 2, wave < 4 ? kBlocks / 2 : kBlocks);
+		float4* half_sums = reinterpret_cast<float4*>(lds + kA) + tile * 256 + lane;
+		if (wave >= 4)
+#pragma unroll
+			for (int q = 0; q < 4; q++) half_sums[q * 64] = make_float4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+		__syncthreads();
+		if (wave < 4) {
+#pragma unroll
+			for (int q = 0; q < 4; q++) {
+				const float4 t = half_sums[q * 64];
+				r[4 * q] = a.step[k].gram * (r[4 * q] + t.x);
+				r[4 * q + 1] = a.step[k].gram * (r[4 * q + 1] + t.y);
+				r[4 * q + 2] = a.step[k].gram * (r[4 * q + 2] + t.z);
+				r[4 * q + 3] = a.step[k].gram * (r[4 * q + 3] + t.w);
+			}
+		}
+		__syncthreads();
+		if (wave < 4) store(r, kA, kRowM, ti, tj);
+		__syncthreads();
+		// B in A's place
+		if (wave < 4) {
+			product(r, kA, kRowM, ti, kA, kRowM, tj, 0, 2);
+			add(r, a.step[k].poly, a.step[k].poly_a, kA, kRowM, ti, tj);
+		}
+		__syncthreads();
+		if (wave < 4) store(r, kA, kRowM, ti, tj);
+		__syncthreads();
+		// X: product u < 2 kBlocks is a tile of B X (written to X^T), the others of X^T B (written to X)
+		const bool last = k + 1 == a.steps;
+		floatx16 x[kShare];
+#pragma unroll
+		for (int i = 0; i < kShare; i++) {
+			const int u = wave + 8 * i, form = u / (2 * kBlocks), rest = u % (2 * kBlocks), mi = rest / kBlocks * 32, ni = rest % kBlocks * 32;
+			if (last && form != (int)a.transposed) continue;
+			if (form == 0) {
+				product(x[i], kA, kRowM, mi, kXt, kRowM, ni, 0, 2);
+				add(x[i], a.step[k].update, a.step[k].update_x, kXt, kRowM, mi, ni);
+			} else {
+				product(x[i], kXt, kRowM, ni, kA, kRowM, mi, 0, 2);
+				add(x[i], a.step[k].update, a.step[k].update_x, kX, kRowX, ni, mi);
+			}
+		}
+		__syncthreads();
+#pragma unroll
+		for (int i = 0; i < kShare; i++) {
+			const int u = wave + 8 * i, form = u / (2 * kBlocks), rest = u % (2 * kBlocks), mi = rest / kBlocks * 32, ni = rest % kBlocks * 32;
+			if (!last) {
+				if (form == 0)
+					store(x[i], kXt, kRowM, mi, ni);
+				else
+					store(x[i], kX, kRowX, ni, mi);
+			} else if (form == (int)a.transposed) {
+				// out has the rows and columns of g: those of X, or of X^T
+				const int rows = a.transposed ? n : m, cols = a.transposed ? m : n, row0 = a.transposed ? ni : mi, col = (a.transposed ? mi : ni) + (lane & 31);
+				float* out = a.out + (size_t)blockIdx.x * m * n;
+#pragma unroll
+				for (int j = 0; j < 16; j++) {
+					const int row = row0 + 8 * (j / 4) + 4 * h + j % 4;
+					if (row < rows && col < cols) out[(size_t)row * cols + col] = x[i][j];
+				}
+			}
+		}
+		__syncthreads();
+	}
+}
+
 // ---- the host's side --------------------------------------------------------------------------------
 
 // max |a s + b s^3 + c s^5| over s in [0, top]: at the end or where the derivative is 0.
@@ -530,6 +731,20 @@ static double scale_for(double bound) {
 	frexp(bound, &e);  // bound <= 2^e
 	return ldexp(1.0, 15 - e);
 }
+
+// The scales of the split matrices, step by step: `next` is the one of X before the first step, then after the last one.
+struct NsScales {
+	double bound = 1.0;  // on the spectral norm of X
+	double x = 0.0, a = 0.0, b = 0.0, next = scale_for(1.0);
+	void step(double ca, double cb, double cc) {
+		x = next;
+		// bounds that rounding does not cross
+		a = scale_for(bound * bound * 1.0001);
+		b = scale_for(largest_square(cb, cc, bound * bound) * 1.0001);
+		bound = largest_quintic(ca, cb, cc, bound) * 1.0001;
+		next = scale_for(bound);
+	}
+};
 
 // The tile of a product whose result is m x n (half of m x m for the symmetric kinds). A larger tile reads less per product
 // but leaves compute units idle. The measured time of a step of 32 columns over all of the result is close to a line in the
@@ -575,6 +790,38 @@ static int ns_product(const NsArgs& args, int tile, size_t p_rows, size_t q_rows
 	return TFHIP_OK;
 }
 
+static int newton_schulz_small(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps) {
+	NsSmallArgs args = {};
+	args.g = g;
+	args.out = out;
+	args.transposed = rows > cols;
+	args.m = (int)(args.transposed ? cols : rows);
+	args.n = (int)(args.transposed ? rows : cols);
+	args.eps = eps;
+	args.steps = steps;
+	NsScales scales;
+	args.scale = (float)scales.next;
+	for (int k = 0; k < steps; k++) {
+		const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
+		scales.step(a, b, c);
+		const double after = k + 1 == steps ? 1.0 : scales.next;
+		args.step[k].gram = (float)(scales.a / (scales.x * scales.x));
+		args.step[k].poly = (float)(c * scales.b / (scales.a * scales.a));
+		args.step[k].poly_a = (float)(b * scales.b / scales.a);
+		args.step[k].update = (float)(after / (scales.b * scales.x));
+		args.step[k].update_x = (float)(a * after / scales.x);
+	}
+	const dim3 grid((unsigned)batch), block(kSmallThreads);
+	if (args.n <= 64)
+		hipLaunchKernelGGL(ns_small_kernel<64>, grid, block, 0, state().stream, args);
+	else if (args.n <= 128)
+		hipLaunchKernelGGL(ns_small_kernel<128>, grid, block, 0, state().stream, args);
+	else
+		hipLaunchKernelGGL(ns_small_kernel<256>, grid, block, 0, state().stream, args);
+	TFHIP_CHECK_LAUNCH();
+	return TFHIP_OK;
+}
+
 // `batch` matrices whose work space fits the arena together.
 static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps, int tile_half, int tile_full, size_t mp, size_t np) {
 	State& s = state();
@@ -595,17 +842,15 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 
 	hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)batch * parts), dim3(256), 0, s.stream, g, partial, elements, parts, (elements & 3) == 0 && ((uintptr_t)g & 15) == 0);
 	TFHIP_CHECK_LAUNCH();
-	double bound = 1.0;
-	double scale_x = scale_for(bound);
+	NsScales scales;
 	const size_t split_groups = (mp / 32 * (np / 32) + 3) / 4, most = (size_t)s.compute_units * 8;
 	hipLaunchKernelGGL(ns_split_kernel, dim3((unsigned)(split_groups < most ? split_groups : most), (unsigned)batch), dim3(256), 0, s.stream, g, (const double*)partial, parts, x, xt, m, n, mp, np, transposed, eps,
-	                   (float)scale_x);
+	                   (float)scales.next);
 	TFHIP_CHECK_LAUNCH();
 	for (int k = 0; k < steps; k++) {
 		const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
-		// bounds that rounding does not cross
-		const double scale_a = scale_for(bound * bound * 1.0001), scale_b = scale_for(largest_square(b, c, bound * bound) * 1.0001);
-		const double next = largest_quintic(a, b, c, bound) * 1.0001, scale_next = scale_for(next);
+		scales.step(a, b, c);
+		const double scale_x = scales.x, scale_a = scales.a, scale_b = scales.b, scale_next = scales.next;
 		NsArgs gram = {};
 		gram.P = gram.Q = x;
 		gram.straight = gram.turned = A;
@@ -662,8 +907,6 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 		t = xt;
 		xt = xt_next;
 		xt_next = t;
-		bound = next;
-		scale_x = scale_next;
 	}
 	return TFHIP_OK;
 }
@@ -688,6 +931,7 @@ extern "C" int tfhip_newton_schulz_f32(const float* g, float* out, size_t batch,
 	if (g != out && words_overlap(g, batch * rows * cols, out, batch * rows * cols)) return fail(TFHIP_ERR_ARG, "Newton-Schulz: g and out overlap without being the same");
 	TFHIP_REQUIRE_INIT();
 	TFHIP_HOLD_DEVICE();
+	if (shorter <= (size_t)kSmallRows && longer <= kSmallCols) return newton_schulz_small(g, out, batch, rows, cols, steps, coefficients, eps);
 	// As many matrices at a time as a work space of 4 GiB holds, at least one.
 	const size_t at_once = batch < 256 ? batch : 256;
 	const int tile_half = ns_tile(shorter, shorter, true, at_once), tile_full = ns_tile(shorter, longer, false, at_once);
