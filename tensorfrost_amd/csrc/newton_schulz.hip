@@ -581,7 +581,6 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 		for (int i = 0; i < 16; i++) low[i] = high[i] = 0.0f;
 		const char* p = lds + P + p0 * p_bytes + (p_bytes == kRowX ? lane_x : lane_m);
 		const char* q = lds + Q + q0 * q_bytes + (q_bytes == kRowX ? lane_x : lane_m);
-#pragma unroll 2
 		for (int kb = kb0; kb < kb1; kb++) {
 			const int at = (kb >> 1) * 256, turn = read_at ^ ((kb & 1) << 7);
 #pragma unroll
