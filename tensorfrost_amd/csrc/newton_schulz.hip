@@ -24,6 +24,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace tfhip {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -497,10 +499,14 @@ __global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const 
 
 // A matrix of at most 64 x 256 (the first and last layers of a small network) stays in the group memory of one compute unit
 // from its norm to its last product: X, its transpose and A (then B in its place) in split form, 2 * 64 * NP * 4 B + 16 KiB. One
-// launch instead of seventeen, which cost 4 to 5 us each whatever they compute.
+// launch instead of seventeen, which take 4 to 5 us each however little they compute. us in the kernels, this one | the seventeen:
+// one matrix of 64 x 64 17 | 65, 64 x 256 40 | 70, 256 x 3 38 | 67; 64 of 64 x 256 43 | 98, 1000 of them 203 | 490.
+// Sixteen waves on 16 x 16 tiles (eight waves on 32 x 32 tiles: 21, 52 and, for the thousand, 268): the products are short, and
+// what takes the time between two barriers is the splitting of the results, some fifteen vector instructions an element, and the
+// group memory's latency; four waves a SIMD cover each other's.
 // The results are written turned (four rows of a lane are four neighbours: 8-byte writes), so X comes from the product
 // X^T B and X^T from B X; the second product costs less than the 2-byte writes of the other orientation.
-constexpr int kSmallRows = 64, kSmallThreads = 512;
+constexpr int kSmallRows = 64, kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
 constexpr size_t kSmallCols = 256;
 
 struct NsSmallArgs {
@@ -524,8 +530,8 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 	constexpr int kX = 0, kXt = kSmallRows * NP * 4, kA = 2 * kXt;  // byte offsets
 	constexpr int kRowX = NP * 4, kRowM = kSmallRows * 4;           // bytes of a row of X; of X^T and A
 	__shared__ __attribute__((aligned(256))) char lds[kA + kSmallRows * kSmallRows * 4];
-	__shared__ double red[kSmallThreads / 64];
-	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+	__shared__ double red[kSmallWaves];
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4;
 	const int m = a.m, n = a.n;
 	const float* g = a.g + (size_t)blockIdx.x * m * n;
 
@@ -548,7 +554,7 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 	__syncthreads();
 	sum = 0.0;
 #pragma unroll
-	for (int w = 0; w < kSmallThreads / 64; w++) sum += red[w];
+	for (int w = 0; w < kSmallWaves; w++) sum += red[w];
 	const double norm = sqrt(sum) + (double)a.eps;
 	const double factor = !isfinite(norm) ? (double)nanf("") : norm > 0.0 ? (double)a.scale / norm : 0.0;
 #pragma unroll
@@ -571,125 +577,128 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 	}
 	__syncthreads();
 
-	// A lane's row of a tile is lane % 32 (tiles begin at multiples of 32), so what small_at exchanges by is the lane's own: the
-	// address of a piece is a lane's part, one exclusive or with a constant, and an offset that the wave shares.
-	const int lane_x = (lane & 31) * kRowX, lane_m = (lane & 31) * kRowM, read_at = ((lane & 15) ^ h) << 4, turned_at = (lane & 15) << 4;
-	// the 32 x 32 tile of rows p0.. of P times rows q0.. of Q over the blocks [kb0, kb1): low products and high ones apart
-	auto product = [&](floatx16& r, int P, int p_bytes, int p0, int Q, int q_bytes, int q0, int kb0, int kb1) {
-		floatx16 low, high;
-#pragma unroll
-		for (int i = 0; i < 16; i++) low[i] = high[i] = 0.0f;
-		const char* p = lds + P + p0 * p_bytes + (p_bytes == kRowX ? lane_x : lane_m);
-		const char* q = lds + Q + q0 * q_bytes + (q_bytes == kRowX ? lane_x : lane_m);
-		for (int kb = kb0; kb < kb1; kb++) {
-			const int at = (kb >> 1) * 256, turn = read_at ^ ((kb & 1) << 7);
-#pragma unroll
-			for (int half = 0; half < 2; half++) {
-				const int hi = at + (turn ^ (half << 5)), lo = at + (turn ^ (half << 5) ^ 64);
-				const half8 p_hi = *reinterpret_cast<const half8*>(p + hi), p_lo = *reinterpret_cast<const half8*>(p + lo);
-				const half8 q_hi = *reinterpret_cast<const half8*>(q + hi), q_lo = *reinterpret_cast<const half8*>(q + lo);
-				low = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_lo, q_hi, low, 0, 0, 0);
-				high = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi, q_hi, high, 0, 0, 0);
-				low = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi, q_lo, low, 0, 0, 0);
-			}
-		}
-#pragma unroll
-		for (int i = 0; i < 16; i++) r[i] = low[i] + high[i];
-		__builtin_amdgcn_sched_barrier(0);  // one product at a time: four interleaved ones do not fit the registers
+	// A lane's row of a tile is lane % 16 (tiles begin at multiples of 16), so what small_at exchanges by is the lane's own: the
+	// address of a piece is a lane's part, one exclusive or with a constant, and an offset that the wave shares. Operands:
+	// 8 columns per quarter of a wave (piece `quarter`). Results: element i of a lane is row 4 quarter + i, column lane % 16.
+	int lane_x = (lane & 15) * kRowX, lane_m = (lane & 15) * kRowM, row_turn = (lane & 15) << 4, read_at = row_turn ^ (quarter << 4);
+	struct Operand {
+		half8 hi, lo;
 	};
-	// r = alpha r + beta D, D turned: D[q0 + lane's column][p0 + rows]
-	auto add = [&](floatx16& r, float alpha, float beta, int D, int d_bytes, int p0, int q0) {
-		const char* d = lds + D + q0 * d_bytes + (d_bytes == kRowX ? lane_x : lane_m) + (p0 >> 6) * 256 + 8 * h;
-		const int turn = turned_at ^ (((p0 >> 5) & 1) << 7);
-#pragma unroll
-		for (int q = 0; q < 4; q++) {
-			const half4 hi = *reinterpret_cast<const half4*>(d + (turn ^ (q << 4))), lo = *reinterpret_cast<const half4*>(d + (turn ^ (q << 4) ^ 64));
-#pragma unroll
-			for (int i = 0; i < 4; i++) r[4 * q + i] = alpha * r[4 * q + i] + beta * ((float)hi[i] + (float)lo[i]);
-		}
+	auto read = [&](int P, int p_bytes, int p0, int kb) {
+		const char* p = lds + P + p0 * p_bytes + (p_bytes == kRowX ? lane_x : lane_m) + (kb >> 1) * 256;
+		const int turn = read_at ^ ((kb & 1) << 7);
+		Operand o;
+		o.hi = *reinterpret_cast<const half8*>(p + turn);
+		o.lo = *reinterpret_cast<const half8*>(p + (turn ^ 64));
+		return o;
 	};
-	auto store = [&](const floatx16& r, int D, int d_bytes, int p0, int q0) {
-		char* d = lds + D + q0 * d_bytes + (d_bytes == kRowX ? lane_x : lane_m) + (p0 >> 6) * 256 + 8 * h;
-		const int turn = turned_at ^ (((p0 >> 5) & 1) << 7);
+	auto multiply = [&](floatx4& low, floatx4& high, const Operand& p, const Operand& q) {
+		low = __builtin_amdgcn_mfma_f32_16x16x32_f16(p.lo, q.hi, low, 0, 0, 0);
+		high = __builtin_amdgcn_mfma_f32_16x16x32_f16(p.hi, q.hi, high, 0, 0, 0);
+		low = __builtin_amdgcn_mfma_f32_16x16x32_f16(p.hi, q.lo, low, 0, 0, 0);
+	};
+	// where a lane's four rows of the tile (p0, q0) lie in D, which holds the result turned: D[q0 + lane's column][p0 + rows]
+	auto place = [&](int D, int d_bytes, int p0, int q0) {
+		const int s = ((p0 >> 5) & 1) * 8 + ((p0 & 16) >> 3) + (quarter >> 1);
+		return lds + D + q0 * d_bytes + (d_bytes == kRowX ? lane_x : lane_m) + (p0 >> 6) * 256 + (row_turn ^ (s << 4)) + (quarter & 1) * 8;
+	};
+	// r = alpha r + beta D
+	auto add = [&](floatx4& r, float alpha, float beta, int D, int d_bytes, int p0, int q0) {
+		const char* d = place(D, d_bytes, p0, q0);
+		const half4 hi = *reinterpret_cast<const half4*>(d), lo = *reinterpret_cast<const half4*>(reinterpret_cast<const char*>(lds) + ((d - lds) ^ 64));
 #pragma unroll
-		for (int q = 0; q < 4; q++) {
-			uint32_t s[4];
+		for (int i = 0; i < 4; i++) r[i] = alpha * r[i] + beta * ((float)hi[i] + (float)lo[i]);
+	};
+	auto store = [&](const floatx4& r, int D, int d_bytes, int p0, int q0) {
+		char* d = place(D, d_bytes, p0, q0);
+		uint32_t s[4];
 #pragma unroll
-			for (int i = 0; i < 4; i++) s[i] = split_pair(r[4 * q + i]);
-			*reinterpret_cast<uint2*>(d + (turn ^ (q << 4))) = make_uint2((s[0] & 0xFFFFu) | (s[1] << 16), (s[2] & 0xFFFFu) | (s[3] << 16));
-			*reinterpret_cast<uint2*>(d + (turn ^ (q << 4) ^ 64)) = make_uint2((s[0] >> 16) | (s[1] & 0xFFFF0000u), (s[2] >> 16) | (s[3] & 0xFFFF0000u));
-		}
+		for (int i = 0; i < 4; i++) s[i] = split_pair(r[i]);
+		*reinterpret_cast<uint2*>(d) = make_uint2((s[0] & 0xFFFFu) | (s[1] << 16), (s[2] & 0xFFFFu) | (s[3] << 16));
+		*reinterpret_cast<uint2*>(lds + ((d - lds) ^ 64)) = make_uint2((s[0] >> 16) | (s[1] & 0xFFFF0000u), (s[2] >> 16) | (s[3] & 0xFFFF0000u));
 	};
 
-	const int tile = wave & 3, ti = (tile >> 1) * 32, tj = (tile & 1) * 32;
-	constexpr int kBlocks = NP / 32;                 // of a row of X
-	constexpr int kShare = NP / 64;                  // products of X and of X^T per wave: 2 * 2 * kBlocks among eight
+	// addresses are worked out anew where they are used: all of them, kept, would take more than the 128 registers of a lane
+	auto forget = [&] { asm volatile("" : "+v"(lane_x), "+v"(lane_m), "+v"(row_turn), "+v"(read_at) :: "memory"); };
+
+	const int ti = (wave >> 2) * 16, tj = (wave & 3) * 16;  // this wave's tile of A and B
+	constexpr int kShare = NP / 32;                         // and its tiles of X and of X^T: 2 * 4 * NP / 16 among sixteen
 	for (int k = 0; k < a.steps; k++) {
-		// A: four tiles, two waves each with half of the columns; the second halves pass through A's own place
-		floatx16 r;
-		product(r, kX, kRowX, ti, kX, kRowX, tj, wave < 4 ? 0 : kBlocks / 2, wave < 4 ? kBlocks / 2 : kBlocks);
-		float4* half_sums = reinterpret_cast<float4*>(lds + kA) + tile * 256 + lane;
-		if (wave >= 4)
-#pragma unroll
-			for (int q = 0; q < 4; q++) half_sums[q * 64] = make_float4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
-		__syncthreads();
-		if (wave < 4) {
-#pragma unroll
-			for (int q = 0; q < 4; q++) {
-				const float4 t = half_sums[q * 64];
-				r[4 * q] = a.step[k].gram * (r[4 * q] + t.x);
-				r[4 * q + 1] = a.step[k].gram * (r[4 * q + 1] + t.y);
-				r[4 * q + 2] = a.step[k].gram * (r[4 * q + 2] + t.z);
-				r[4 * q + 3] = a.step[k].gram * (r[4 * q + 3] + t.w);
-			}
-		}
-		__syncthreads();
-		if (wave < 4) store(r, kA, kRowM, ti, tj);
+		forget();
+		floatx4 low = {0.0f, 0.0f, 0.0f, 0.0f}, high = low;
+#pragma unroll 4
+		for (int kb = 0; kb < NP / 32; kb++) multiply(low, high, read(kX, kRowX, ti, kb), read(kX, kRowX, tj, kb));
+		floatx4 r = a.step[k].gram * (low + high);
+		store(r, kA, kRowM, ti, tj);
 		__syncthreads();
 		// B in A's place
-		if (wave < 4) {
-			product(r, kA, kRowM, ti, kA, kRowM, tj, 0, 2);
-			add(r, a.step[k].poly, a.step[k].poly_a, kA, kRowM, ti, tj);
-		}
+		low = high = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+		for (int kb = 0; kb < 2; kb++) multiply(low, high, read(kA, kRowM, ti, kb), read(kA, kRowM, tj, kb));
+		r = low + high;
+		add(r, a.step[k].poly, a.step[k].poly_a, kA, kRowM, ti, tj);
 		__syncthreads();
-		if (wave < 4) store(r, kA, kRowM, ti, tj);
+		store(r, kA, kRowM, ti, tj);
 		__syncthreads();
-		// X: product u < 2 kBlocks is a tile of B X (written to X^T), the others of X^T B (written to X)
+		// X: waves 0 .. 7 the tiles of B X (written to X^T), the others those of X^T B (written to X); a wave has one of the four
+		// rows of tiles of B and every second one of X^T
 		const bool last = k + 1 == a.steps;
-		floatx16 x[kShare];
+		const int form = wave >> 3, mi = (wave & 3) * 16, n0 = (wave >> 2) & 1;
+		floatx4 x[kShare];
+		auto multiply_x = [&](auto which) {
+			constexpr bool kTurned = which;
+			const Operand b0 = read(kA, kRowM, mi, 0), b1 = read(kA, kRowM, mi, 1);
 #pragma unroll
-		for (int i = 0; i < kShare; i++) {
-			const int u = wave + 8 * i, form = u / (2 * kBlocks), rest = u % (2 * kBlocks), mi = rest / kBlocks * 32, ni = rest % kBlocks * 32;
-			if (last && form != (int)a.transposed) continue;
-			if (form == 0) {
-				product(x[i], kA, kRowM, mi, kXt, kRowM, ni, 0, 2);
-				add(x[i], a.step[k].update, a.step[k].update_x, kXt, kRowM, mi, ni);
-			} else {
-				product(x[i], kXt, kRowM, ni, kA, kRowM, mi, 0, 2);
-				add(x[i], a.step[k].update, a.step[k].update_x, kX, kRowX, ni, mi);
-			}
-		}
-		__syncthreads();
-#pragma unroll
-		for (int i = 0; i < kShare; i++) {
-			const int u = wave + 8 * i, form = u / (2 * kBlocks), rest = u % (2 * kBlocks), mi = rest / kBlocks * 32, ni = rest % kBlocks * 32;
-			if (!last) {
-				if (form == 0)
-					store(x[i], kXt, kRowM, mi, ni);
-				else
-					store(x[i], kX, kRowX, ni, mi);
-			} else if (form == (int)a.transposed) {
-				// out has the rows and columns of g: those of X, or of X^T
-				const int rows = a.transposed ? n : m, cols = a.transposed ? m : n, row0 = a.transposed ? ni : mi, col = (a.transposed ? mi : ni) + (lane & 31);
-				float* out = a.out + (size_t)blockIdx.x * m * n;
-#pragma unroll
-				for (int j = 0; j < 16; j++) {
-					const int row = row0 + 8 * (j / 4) + 4 * h + j % 4;
-					if (row < rows && col < cols) out[(size_t)row * cols + col] = x[i][j];
+			for (int i = 0; i < kShare; i++) {
+				const int ni = (2 * i + n0) * 16;
+				low = high = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+				const Operand x0 = read(kXt, kRowM, ni, 0), x1 = read(kXt, kRowM, ni, 1);
+				if constexpr (kTurned) {
+					multiply(low, high, x0, b0);
+					multiply(low, high, x1, b1);
+				} else {
+					multiply(low, high, b0, x0);
+					multiply(low, high, b1, x1);
 				}
+				x[i] = low + high;
+				if constexpr (kTurned)
+					add(x[i], a.step[k].update, a.step[k].update_x, kX, kRowX, ni, mi);
+				else
+					add(x[i], a.step[k].update, a.step[k].update_x, kXt, kRowM, mi, ni);
+				forget();
+			}
+		};
+		auto store_x = [&](auto which) {
+#pragma unroll
+			for (int i = 0; i < kShare; i++) {
+				const int ni = (2 * i + n0) * 16;
+				if constexpr (which)
+					store(x[i], kX, kRowX, ni, mi);
+				else
+					store(x[i], kXt, kRowM, mi, ni);
+				forget();
+			}
+		};
+		if (!last) {
+			form ? multiply_x(std::true_type()) : multiply_x(std::false_type());
+			__syncthreads();
+			form ? store_x(std::true_type()) : store_x(std::false_type());
+			__syncthreads();
+		} else if (form == (int)a.transposed) {
+			form ? multiply_x(std::true_type()) : multiply_x(std::false_type());
+			// out has the rows and columns of g: those of X, or of X^T
+			const int rows = a.transposed ? n : m, cols = a.transposed ? m : n;
+			float* out = a.out + (size_t)blockIdx.x * m * n;
+			int row = 4 * quarter, col = lane & 15;
+			asm volatile("" : "+v"(row), "+v"(col));
+#pragma unroll
+			for (int i = 0; i < kShare; i++) {
+				const int ni = (2 * i + n0) * 16, row0 = (a.transposed ? ni : mi) + row, col0 = (a.transposed ? mi : ni) + col;
+#pragma unroll
+				for (int j = 0; j < 4; j++)
+					if (row0 + j < rows && col0 < cols) out[(row0 + j) * cols + col0] = x[i][j];
 			}
 		}
-		__syncthreads();
 	}
 }
 
