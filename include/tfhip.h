@@ -249,8 +249,8 @@ int tfhip_sgemm_batched(int layout, const float* A, const float* B, float* C, si
  * the mean and norm reductions, loads with computed indices and atomic adds (Compiler/Implementations.cpp:243-303,
  * 451-488), and its optimisers end at the element-wise update (Python/TensorFrost/optimizers.py:104-167). All matrices
  * are dense row-major fp32; every sum is held in fp32 or wider, in an order that does not change from run to run.
- * Several host threads may call these and the primitives above at once: the launches of one call stay together on the
- * library's stream. The library's device is made current for the length of a call.
+ * Several host threads may call these, the primitives above and tfhip_graph_launch at once: the launches of one call stay
+ * together on the library's stream. The library's device is made current for the length of a call.
  * They may be recorded into a graph (run the same work once before, so that the scratch buffer has its size). */
 
 /* y[r,c] = (x[r,c] - mean[r]) * rstd[r] * weight[c] + bias[c], mean[r] = mean_c x[r,:], rstd[r] = 1 / sqrt(mean_c (x[r,:] -
@@ -275,9 +275,11 @@ int tfhip_embedding_rows_backward_f32(const int32_t* tokens, const float* dy, fl
 
 /* Orthogonalises `batch` matrices [rows, cols] that follow each other: X = G / (|G|_F + eps), then `steps` times (1 to 64)
  * A = X X^T, X <- a X + (b A + c A^2) X with that step's three coefficients (host memory, 3 * steps finite floats: a, b, c
- * of the first step first); with rows > cols the same on the transposed matrix. A matrix of zeros stays zero; one with an infinity or NaN comes out
- * as NaN. g == out is allowed, any other overlap is refused. At most 32768 on the shorter side, 2^31 - 1
- * elements in a matrix and 65535 matrices; batch == 0 is a no-op. */
+ * of the first step first); with rows > cols the same on the transposed matrix. Operands of the products keep 22 bits;
+ * elements below 2^-12 of the bound on their matrix keep an absolute error of 2^-40 of it, so with |G|_F far below eps the
+ * small X of the first steps is known to 2^-40 only. A matrix of zeros stays zero; one with an infinity or NaN comes out as
+ * NaN. g == out is allowed, any other overlap is refused. At most 32768 on the shorter side, 2^23 - 1 on the longer one,
+ * 2^31 - 1 elements in a matrix and 65535 matrices; batch == 0 is a no-op. */
 int tfhip_newton_schulz_f32(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps);
 
 #ifdef __cplusplus

@@ -758,6 +758,7 @@ int tfhip_sync(void) {
 
 int tfhip_graph_begin(void) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	State& s = state();
 	if (s.capturing) return fail(TFHIP_ERR_STATE, "a graph is already being recorded");
 	g_recorded_arguments.clear();
@@ -769,6 +770,7 @@ int tfhip_graph_begin(void) {
 
 int tfhip_graph_end(tfhip_graph_t* out) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	State& s = state();
 	if (!s.capturing) return fail(TFHIP_ERR_STATE, "no graph is being recorded");
 	s.capturing = false;
@@ -806,6 +808,7 @@ int tfhip_graph_node_count(tfhip_graph_t graph, size_t* nodes) {
 
 int tfhip_graph_launch(tfhip_graph_t graph) {
 	TFHIP_REQUIRE_INIT();
+	TFHIP_HOLD_DEVICE();
 	if (!graph || !graph->exec) return fail(TFHIP_ERR_ARG, "graph handle is null");
 	TFHIP_REFUSE_WHILE_RECORDING("launching a graph");
 	TFHIP_CHECK(hipGraphLaunch(graph->exec, state().stream));
@@ -814,6 +817,7 @@ int tfhip_graph_launch(tfhip_graph_t graph) {
 
 int tfhip_graph_destroy(tfhip_graph_t graph) {
 	if (!graph) return TFHIP_OK;
+	CallGuard guard;
 	if (state().initialized) hipStreamSynchronize(state().stream);
 	if (graph->exec) hipGraphExecDestroy(graph->exec);
 	if (graph->graph) hipGraphDestroy(graph->graph);

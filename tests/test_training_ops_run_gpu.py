@@ -264,6 +264,38 @@ def test_two_threads_at_once(rt):
     assert same(calls[0].results(), wants[0]) and same(calls[1].results(), wants[1])
 
 
+def test_a_graph_launched_beside_another_threads_calls(rt):
+    """The graph's work and the other thread's calls use the same scratch buffer: neither may begin inside the other."""
+    recorded, eager = Calls(rt, 6000, 150, 300, seed=6), Calls(rt, 7000, 300, 90, seed=7)
+    wants = []
+    for c in (recorded, eager):
+        c.run()
+        wants.append(c.results())
+    graph = rt.Graph()
+    with graph:
+        recorded.run()
+    for c in (recorded, eager):
+        c.clear()
+    errors = []
+
+    def work(step):
+        try:
+            for _ in range(30):
+                step()
+        except Exception as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(step,)) for step in (graph.launch, eager.run)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    rt.synchronize()
+    assert not errors
+    assert same(recorded.results(), wants[0]) and same(eager.results(), wants[1])
+    graph.destroy()
+
+
 def test_memory_of_another_library_and_its_stream(rt):
     torch = pytest.importorskip("torch")
     stream = torch.cuda.Stream()
