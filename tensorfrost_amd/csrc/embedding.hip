@@ -404,7 +404,7 @@ static int embedding_sums(const uint32_t* keys, const uint32_t* order, const flo
 // ---- few positions ----------------------------------------------------------------------------------------
 
 // Up to kFewPositions positions of a table of moderate size in one launch, without an order of all of them: a group owns
-// kFewRows rows of the table, looks through all tokens, lists the positions of its rows in their order (8 waves, a ballot
+// kFewRows rows of the table, looks through all tokens (one per thread), lists the positions of its rows in their order (8 waves, a ballot
 // each) and adds up the rows' dy. A wave takes a row with few positions; a row with more than kFewAlone is cut into eight
 // parts of neighbouring positions, one per wave, added in their order at the end. Rows without positions get their zeros on
 // the way. Against the three launches below (counting, sums, joins; us in the kernels): 500 x 250 over 1009 rows 8.0 | 14.0,
@@ -413,76 +413,71 @@ static int embedding_sums(const uint32_t* keys, const uint32_t* order, const flo
 constexpr uint32_t kFewPositions = 512;
 constexpr size_t kFewVocab = 8192, kFewCols = 512;
 constexpr int kFewRows = 8, kFewWaves = 8, kFewAlone = 32;
+static_assert(kFewWaves * 64 == kFewPositions, "a thread per position");
 
 template <int VEC>
 __global__ __launch_bounds__(kFewWaves * 64) void embedding_few_kernel(const int32_t* __restrict__ tokens, const float* __restrict__ dy, float* __restrict__ dtable, uint32_t n, uint32_t vocab,
                                                                        size_t cols, float scale) {
 	typedef typename Floats<VEC>::type Vec;
 	__shared__ uint16_t list[kFewRows][kFewPositions];
-	__shared__ uint32_t found[kFewRows][kFewWaves];  // of one turn's tokens
+	__shared__ uint32_t found[kFewRows][kFewWaves];
 	__shared__ Vec parts[kFewWaves][64];
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	for (uint64_t v0 = (uint64_t)blockIdx.x * kFewRows; v0 < vocab; v0 += (uint64_t)gridDim.x * kFewRows) {
-		uint32_t count[kFewRows];  // the same in every thread
+	const uint32_t v0 = blockIdx.x * kFewRows;
+	const uint32_t token = threadIdx.x < n ? (uint32_t)tokens[threadIdx.x] : 0xFFFFFFFFu;  // names no row
+	const uint32_t mine = token < vocab ? token - v0 : 0xFFFFFFFFu;                         // its row of this group's, if below kFewRows
+	uint64_t votes[kFewRows];
+	uint32_t count[kFewRows];  // the same in every thread
 #pragma unroll
-		for (int r = 0; r < kFewRows; r++) count[r] = 0;
-		for (uint32_t base = 0; base < n; base += kFewWaves * 64) {
-			const uint32_t i = base + threadIdx.x;
-			const uint32_t mine = i < n ? (uint32_t)tokens[i] - (uint32_t)v0 : 0xFFFFFFFFu;
-			const bool real = i < n && (uint64_t)(uint32_t)tokens[i < n ? i : 0] < vocab;
-			uint64_t votes[kFewRows];
+	for (int r = 0; r < kFewRows; r++) {
+		votes[r] = __ballot(mine == (uint32_t)r);
+		if (lane == 0) found[r][wave] = __popcll(votes[r]);
+	}
+	__syncthreads();
 #pragma unroll
-			for (int r = 0; r < kFewRows; r++) {
-				votes[r] = __ballot(real && mine == (uint32_t)r);
-				if (lane == 0) found[r][wave] = __popcll(votes[r]);
-			}
-			__syncthreads();
+	for (int r = 0; r < kFewRows; r++) {
+		uint32_t at = 0;
+		count[r] = 0;
 #pragma unroll
-			for (int r = 0; r < kFewRows; r++) {
-				uint32_t at = count[r];
-#pragma unroll
-				for (int w = 0; w < kFewWaves; w++) {
-					const uint32_t f = found[r][w];
-					at += w < wave ? f : 0;
-					count[r] += f;
-				}
-				if (real && mine == (uint32_t)r) list[r][at + __popcll(votes[r] & ((1ull << lane) - 1))] = (uint16_t)i;
-			}
-			__syncthreads();
+		for (int w = 0; w < kFewWaves; w++) {
+			const uint32_t f = found[r][w];
+			at += w < wave ? f : 0;
+			count[r] += f;
 		}
+		if (mine == (uint32_t)r) list[r][at + __popcll(votes[r] & ((1ull << lane) - 1))] = (uint16_t)threadIdx.x;
+	}
+	__syncthreads();
 #pragma unroll
-		for (int r = 0; r < kFewRows; r++) {
-			if (v0 + r >= vocab) break;
-			const bool shared = count[r] > kFewAlone;
-			if (!shared && r % kFewWaves != wave) continue;
-			// this wave's positions of the row
-			const uint32_t share = (count[r] + kFewWaves - 1) / kFewWaves;
-			const uint32_t first = shared ? wave * share : 0, last = shared ? (first + share < count[r] ? first + share : count[r]) : count[r];
-			for (size_t c0 = 0; c0 < cols; c0 += 64 * VEC) {
-				const size_t c = c0 + (size_t)lane * VEC;
-				Vec sum = Vec(0.0f);
-				if (c < cols)
-					for (uint32_t p0 = first; p0 < last; p0 += kSumRows) {
-						Vec v[kSumRows];
+	for (int r = 0; r < kFewRows; r++) {
+		if (v0 + r >= vocab) break;
+		const bool shared = count[r] > kFewAlone;
+		if (!shared && r % kFewWaves != wave) continue;
+		// this wave's positions of the row
+		const uint32_t share = (count[r] + kFewWaves - 1) / kFewWaves;
+		const uint32_t first = shared ? wave * share : 0, last = shared ? (first + share < count[r] ? first + share : count[r]) : count[r];
+		for (size_t c0 = 0; c0 < cols; c0 += 64 * VEC) {
+			const size_t c = c0 + (size_t)lane * VEC;
+			Vec sum = Vec(0.0f);
+			if (c < cols)
+				for (uint32_t p0 = first; p0 < last; p0 += kSumRows) {
+					Vec v[kSumRows];
 #pragma unroll
-						for (int u = 0; u < kSumRows; u++) v[u] = *reinterpret_cast<const Vec*>(dy + (size_t)list[r][p0 + u < last ? p0 + u : p0] * cols + c);
+					for (int u = 0; u < kSumRows; u++) v[u] = *reinterpret_cast<const Vec*>(dy + (size_t)list[r][p0 + u < last ? p0 + u : p0] * cols + c);
 #pragma unroll
-						for (int u = 0; u < kSumRows; u++)
-							if (p0 + u < last) sum += v[u];
-					}
-				if (shared) {
-					parts[wave][lane] = sum;
-					__syncthreads();
-					if (wave == 0) {
-#pragma unroll
-						for (int w = 1; w < kFewWaves; w++) sum += parts[w][lane];
-					}
+					for (int u = 0; u < kSumRows; u++)
+						if (p0 + u < last) sum += v[u];
 				}
-				if ((!shared || wave == 0) && c < cols) __builtin_nontemporal_store(sum * scale, reinterpret_cast<Vec*>(dtable + (size_t)(v0 + r) * cols + c));
-				if (shared) __syncthreads();
+			if (shared) {
+				parts[wave][lane] = sum;
+				__syncthreads();
+				if (wave == 0) {
+#pragma unroll
+					for (int w = 1; w < kFewWaves; w++) sum += parts[w][lane];
+				}
 			}
+			if ((!shared || wave == 0) && c < cols) __builtin_nontemporal_store(sum * scale, reinterpret_cast<Vec*>(dtable + (size_t)(v0 + r) * cols + c));
+			if (shared) __syncthreads();
 		}
-		__syncthreads();  // the list is read: the next rows may overwrite it
 	}
 }
 
@@ -532,8 +527,7 @@ extern "C" int tfhip_embedding_rows_backward_f32(const int32_t* tokens, const fl
 	if (n == 0) return tfhip_fill_u32(dtable, 0u, vocab * cols);
 	if (n <= kFewPositions && vocab <= kFewVocab && cols <= kFewCols) {
 		const RowShape r = row_shape(cols, dy, dtable);
-		const size_t most = (size_t)s.compute_units * 16, want = (vocab + kFewRows - 1) / kFewRows;
-		const dim3 grid((unsigned)(want < most ? want : most)), block(kFewWaves * 64);
+		const dim3 grid((unsigned)((vocab + kFewRows - 1) / kFewRows)), block(kFewWaves * 64);
 		switch (r.vec) {
 			case 4: hipLaunchKernelGGL(embedding_few_kernel<4>, grid, block, 0, s.stream, tokens, dy, dtable, (uint32_t)n, (uint32_t)vocab, cols, scale); break;
 			case 2: hipLaunchKernelGGL(embedding_few_kernel<2>, grid, block, 0, s.stream, tokens, dy, dtable, (uint32_t)n, (uint32_t)vocab, cols, scale); break;

@@ -124,6 +124,25 @@ def test_nan_and_infinity_reach_only_the_rows_that_hold_them(rt):
     assert (~np.isfinite(got)).sum() == 1
 
 
+# on both sides of the sizes at which another kernel takes over: 512 positions, 8192 rows, 512 columns, 4096 and 131072 positions
+@pytest.mark.parametrize("shape", [(511, 8191, 511), (512, 8192, 512), (512, 8193, 512), (513, 8192, 64), (512, 9, 513), (512, 7, 512), (65, 8, 130), (4095, 300, 20), (4096, 300, 20), (4097, 300, 20),
+                                   (131072, 300, 4), (131073, 300, 4)])
+@pytest.mark.parametrize("kind", ["skewed", "one token", "a long run and a short one", "none"])
+def test_gradient_beside_the_sizes_where_the_kernel_changes(rt, shape, kind):
+    n, vocab, cols = shape
+    rng = np.random.default_rng([n, vocab, cols, 1])
+    t = {"skewed": lambda: tokens_for(n, vocab, 6, pad=0.1), "one token": lambda: np.full(n, vocab // 2, np.int32),
+         "a long run and a short one": lambda: np.where(np.arange(n) % 9 == 4, 0, vocab - 1).astype(np.int32), "none": lambda: np.full(n, vocab, np.int32)}[kind]()
+    dy = rng.integers(-4, 5, (n, cols)).astype(np.float32)
+    dy[(t < 0) | (t >= vocab)] = np.nan  # nobody's
+    d = rt.DeviceBuffer(vocab * cols + 64)
+    d.fill(0x7FC00000)
+    rt.embedding_rows_backward(rt.DeviceBuffer.from_numpy(t), rt.DeviceBuffer.from_numpy(dy), d, n, vocab, cols, scale=0.5)
+    got = d.numpy(np.float32)
+    assert np.array_equal(got[: vocab * cols].reshape(vocab, cols), (0.5 * gradient(t, dy, vocab)).astype(np.float32))
+    assert np.isnan(got[vocab * cols:]).all()
+
+
 def test_no_tokens(rt):
     d = rt.DeviceBuffer.from_numpy(np.ones(12, np.float32))
     rt.embedding_rows(d, d, rt.DeviceBuffer(4), 0, 3, 4)
