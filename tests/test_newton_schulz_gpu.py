@@ -95,6 +95,25 @@ def test_a_batch_is_its_matrices_one_by_one(rt, batch, shape):
         assert np.linalg.norm(got[k] - want) <= 200 * e(max(shape)) * np.linalg.norm(want)
 
 
+# on both sides of the sizes at which another kernel takes over, in both orientations
+@pytest.mark.parametrize("shape", [(64, 65), (64, 128), (64, 129), (64, 256), (64, 257), (65, 65), (65, 256), (1, 256), (1, 257), (17, 31), (48, 250)])
+@pytest.mark.parametrize("tall", [False, True])
+def test_beside_the_sizes_where_the_kernel_changes(rt, shape, tall):
+    batch = 3
+    g = np.stack([make(*shape, seed=20 + k) for k in range(batch)])
+    g = np.ascontiguousarray(np.swapaxes(g, 1, 2)) if tall else g
+    rows, cols = g.shape[1:]
+    triples = ((3.9, -8.1, 4.9), QUINTIC, (1.875, -1.25, 0.375))
+    got = run(rt, g, batch=batch, steps=3, coefficients=triples)
+    b = rt.DeviceBuffer.from_numpy(g)
+    rt.newton_schulz(b, b, rows, cols, steps=3, batch=batch, coefficients=triples)
+    assert np.array_equal(b.numpy(np.float32, g.shape), got)  # in place
+    for k in range(batch):
+        want = newton_schulz64(g[k], 3, triples)
+        # at most 3.9 * 3.4445 * 1.875 times an error of the first step, three steps' worth of them
+        assert np.linalg.norm(got[k] - want) <= 3 * 25.2 * e(max(shape)) * np.linalg.norm(want)
+
+
 @pytest.mark.parametrize("shape", [(40, 40), (64, 200), (300, 128)])
 def test_other_coefficients_and_step_counts(rt, shape):
     g = make(*shape, seed=3)
