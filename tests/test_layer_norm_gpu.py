@@ -128,6 +128,22 @@ def test_backward_against_float64(rt, shape):
     assert np.array_equal(xb.numpy(np.float32, shape), got) and np.array_equal(one_w.numpy(), dw.numpy()) and np.array_equal(one_b.numpy(), db.numpy())
 
 
+# rows that end one, two and three elements into a vector, on both sides of the widths at which another kernel takes over
+@pytest.mark.parametrize("cols", [1023, 1025, 2047, 2049, 4093, 4095, 4097, 4098, 4099, 8190, 8193, 8195, 16381, 16382, 16383, 16385, 16386, 24577, 24579])
+@pytest.mark.parametrize("rows", [1, 7])
+def test_rows_that_end_inside_a_vector(rt, rows, cols):
+    test_forward_against_float64(rt, (rows, cols))
+    test_backward_against_float64(rt, (rows, cols))
+    x, w, _, dy = make(rows, cols, seed=2)
+    xb, wb, dyb, dx = (rt.DeviceBuffer.from_numpy(a) for a in (x, w, dy, np.zeros_like(x)))
+    mean, rstd = rt.DeviceBuffer(rows), rt.DeviceBuffer(rows)
+    rt.layer_norm_rows(xb, wb, None, dx, rows, cols, mean=mean, rstd=rstd)
+    rt.layer_norm_rows_backward(xb, dyb, wb, mean, rstd, rows, cols, dx=dx)
+    want = dx.numpy(np.float32, x.shape)
+    rt.layer_norm_rows_backward(xb, dyb, wb, mean, rstd, rows, cols, dx=dyb)  # the gradient in dy's place: the same words
+    assert np.array_equal(dyb.numpy(np.float32, x.shape), want)
+
+
 @pytest.mark.parametrize("shape", [(9, 64), (130, 256), (33, 1024), (5, 4096), (3, 20000)])
 @pytest.mark.parametrize("odd", ["x", "weight", "out", "dy"])
 def test_addresses_that_are_only_word_aligned(rt, shape, odd):
