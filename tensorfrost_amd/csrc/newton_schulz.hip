@@ -24,6 +24,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace tfhip {
@@ -175,6 +176,9 @@ struct NsArgs {
 	uint32_t k_blocks;          // blocks of a row of P and Q
 	uint32_t tiles_p, tiles_q;
 	uint32_t band;  // tile rows of a patch
+	uint32_t whole;   // tiles that one group each works on; the others are cut along k
+	uint32_t cuts;    // into so many parts
+	float4* partial;  // the parts' sums
 	float alpha;  // what an element of the accumulator is multiplied with
 	float beta;   // ... and an element of the addend
 };
@@ -198,11 +202,14 @@ __device__ __forceinline__ void wait_loads() {
 // the band before the next), so that a die reads as few different rows of P and Q as its share of the work allows.
 // The symmetric products list each pair of tile rows once as (r, r + c modulo n), c = 0 .. n / 2 (for even n only half of
 // the r at c = n / 2), which makes the triangle a rectangle of n rows.
+// The tiles that are cut follow the whole ones.
+__device__ __forceinline__ uint32_t whole_tile_of_group(const NsArgs& g) {
+	const uint32_t q = g.whole >> 3, rem = g.whole & 7, die = blockIdx.x & 7;
+	return die * q + (die < rem ? die : rem) + (blockIdx.x >> 3);
+}
 template <int KIND>
-__device__ __forceinline__ void tile_of_group(const NsArgs& g, uint32_t& tp, uint32_t& tq) {
+__device__ __forceinline__ void place_of_tile(const NsArgs& g, uint32_t t, uint32_t& tp, uint32_t& tq) {
 	constexpr bool kHalf = KIND == kNsGram || KIND == kNsPoly;
-	const uint32_t q = gridDim.x >> 3, rem = gridDim.x & 7, die = blockIdx.x & 7;
-	const uint32_t t = die * q + (die < rem ? die : rem) + (blockIdx.x >> 3);
 	const uint32_t rows = g.tiles_p, cols = kHalf ? (g.tiles_p + 1) / 2 : g.tiles_q;
 	uint32_t r, c;
 	if (!kHalf || t < rows * cols) {
@@ -273,6 +280,7 @@ __global__ __launch_bounds__(WP* WQ* KS * 64) void ns_product_kernel(const NsArg
 	constexpr int kWaves = WP * WQ * KS;
 	constexpr int kRows = TP + TQ;
 	constexpr int kStage = kRows * kNsBlock;             // bytes of one block of columns of both operands
+	constexpr bool kCut = TP <= 128;
 	constexpr int kLoads = kRows / (8 * kWaves);         // a load of a wave brings 8 rows
 	constexpr int SP = TP / WP / 32, SQ = TQ / WQ / 32;  // 32 x 32 tiles of a wave
 	static_assert(kLoads * 8 * kWaves == kRows, "rows divide among the waves");
@@ -283,10 +291,19 @@ __global__ __launch_bounds__(WP* WQ* KS * 64) void ns_product_kernel(const NsArg
 	const int lane = threadIdx.x & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	uint32_t tp, tq;
-	tile_of_group<KIND>(g, tp, tq);
+	uint32_t first = 0, steps = g.k_blocks;
+	const bool part = kCut && blockIdx.x >= g.whole;
+	if (part) {
+		const uint32_t at = blockIdx.x - g.whole, cut = at % g.cuts;
+		place_of_tile<KIND>(g, g.whole + at / g.cuts, tp, tq);
+		first = cut * g.k_blocks / g.cuts;
+		steps = (cut + 1) * g.k_blocks / g.cuts - first;
+	} else {
+		place_of_tile<KIND>(g, whole_tile_of_group(g), tp, tq);
+	}
 	const size_t stride = (size_t)g.k_blocks * kNsBlock;
-	const char* P = g.P + blockIdx.y * g.batch_p + (size_t)tp * TP * stride;
-	const char* Q = g.Q + blockIdx.y * g.batch_q + (size_t)tq * TQ * stride;
+	const char* P = g.P + blockIdx.y * g.batch_p + (size_t)tp * TP * stride + first * kNsBlock;
+	const char* Q = g.Q + blockIdx.y * g.batch_q + (size_t)tq * TQ * stride + first * kNsBlock;
 
 	// Row r of a stage lies at 128 r; its 16-byte piece c at place c ^ (r / 2 % 8), so that the 16 lanes that read one
 	// piece of 16 rows together meet 16 different quarters of the banks.
@@ -318,7 +335,6 @@ __global__ __launch_bounds__(WP* WQ* KS * 64) void ns_product_kernel(const NsArg
 	const char* frag_q = lds + (TP + wq * SQ * 32 + (lane & 31)) * kNsBlock;
 
 	// A ring of STAGES stages: while one is multiplied, the next STAGES - 1 are on their way.
-	const uint32_t steps = g.k_blocks;
 	uint32_t fetched = 0, fill = 0;  // steps asked for; where the next one goes
 	auto fetch = [&]() {
 #pragma unroll
@@ -400,10 +416,48 @@ __global__ __launch_bounds__(WP* WQ* KS * 64) void ns_product_kernel(const NsArg
 					v[4 * q + 3] += t.w;
 				}
 			}
+			if (part) {
+				// [tile, part][wave of a set][32 x 32 tile][4 quarters][lane]
+				float4* to = g.partial + ((((size_t)(blockIdx.x - g.whole) * WP * WQ + wave) * SP + i) * SQ + j) * 256 + lane;
+#pragma unroll
+				for (int q = 0; q < 4; q++) to[q * 64] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+				continue;
+			}
 			Addend a;
 			if (KIND != kNsGram) load_addend(g, a, row0, col0);
 			finish_tile<KIND>(g, v, a, row0, col0, tp == tq, corner);
 		}
+}
+
+// The tiles that were cut: the parts' sums in their order, and then as a group with the whole tile would go on. A wave per 32 x 32
+// tile. T, WP, WQ as in ns_product_kernel.
+template <int T, int WP, int WQ, int KIND>
+__global__ __launch_bounds__(256) void ns_join_kernel(const NsArgs g) {
+	__shared__ uint32_t corner[4][32 * 33];
+	constexpr int SP = T / WP / 32, SQ = T / WQ / 32, kTiles = T / 32 * T / 32, kGroups = kTiles / 4;  // 32 x 32 tiles, groups for them
+	const int lane = threadIdx.x & 63, corner_of = threadIdx.x >> 6;
+	const uint32_t at = blockIdx.x / kGroups, sub = (blockIdx.x % kGroups) * 4 + corner_of;
+	uint32_t tp, tq;
+	place_of_tile<KIND>(g, g.whole + at, tp, tq);
+	const uint32_t wave = sub / (SP * SQ), i = sub / SQ % SP, j = sub % SQ;
+	const uint32_t row0 = tp * T + (wave / WQ * SP + i) * 32, col0 = tq * T + (wave % WQ * SQ + j) * 32;
+	Addend addend;
+	if (KIND != kNsGram) load_addend(g, addend, row0, col0);
+	const float4* from = g.partial + ((size_t)at * g.cuts * kTiles + sub) * 256 + lane;
+	float v[16];
+#pragma unroll
+	for (int r = 0; r < 16; r++) v[r] = 0.0f;
+#pragma unroll 4
+	for (uint32_t c = 0; c < g.cuts; c++, from += kTiles * 256)
+#pragma unroll
+		for (int q = 0; q < 4; q++) {
+			const float4 t = from[q * 64];
+			v[4 * q] += t.x;
+			v[4 * q + 1] += t.y;
+			v[4 * q + 2] += t.z;
+			v[4 * q + 3] += t.w;
+		}
+	finish_tile<KIND>(g, v, addend, row0, col0, tp == tq, corner[corner_of]);
 }
 
 // Few tiles: what counts is the way from the first load to the last store. A group of eight waves owns a 32 x 32 tile; each
@@ -420,7 +474,7 @@ __global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const 
 	const int lane = threadIdx.x & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	uint32_t tp, tq;
-	tile_of_group<KIND>(g, tp, tq);
+	place_of_tile<KIND>(g, whole_tile_of_group(g), tp, tq);
 	const size_t stride = (size_t)g.k_blocks * kNsBlock;
 	const uint32_t block = wave >> 1;
 	const char* src = (wave & 1 ? g.Q + blockIdx.y * g.batch_q + (size_t)tq * T * stride : g.P + blockIdx.y * g.batch_p + (size_t)tp * T * stride) + block * kNsBlock;
@@ -778,15 +832,56 @@ static int ns_tile(size_t m, size_t n, bool half, size_t batch) {
 	return best;
 }
 
+// Tiles that are left over when every compute unit has had the same number keep few units busy for the time of a whole tile:
+// into how many parts along k each of them is cut (1: not), `left` receiving their number. By the measured time of a step of
+// the tiles that a unit works on, the parts' way through memory at 5 TB/s and 6 us for the join; it has to save a seventh of
+// the round. us per product, cut, with the join | whole: A of 4096 x 4096 (528 tiles of 128) 202 | 239, of 3000 x 3000 (300)
+// 96 | 115, X of 3000 x 3000 (576) 171 | 201; not cut: A of 3500 x 3500 (406) 148 | 144. Three tiles of 64 share a unit and the
+// first two hardly slow each other, so those are cut from two rounds on: A of 2000 x 4100 (528 tiles of 64) 76 | 88, of 2048 x 2048
+// 42.5 | 44; not cut: A of 1500 x 3000 (300) 44 | 41.
+static unsigned ns_cuts(size_t tiles, int tile, uint32_t k_blocks, size_t batch, size_t& left) {
+	const size_t units = state().compute_units;
+	left = tiles % units;
+	if (batch != 1 || left == 0 || !(tile == 128 || (tile == 64 && tiles >= 2 * units))) return 1;
+	const double round = (tile == 128 ? 0.69 : 0.28) * k_blocks, part = tile * tile * 1.6e-6;  // us
+	double least = 0.85 * round;
+	unsigned best = 1;
+	for (unsigned c = 2; c <= 16 && k_blocks / c >= 4; c++) {
+		const double time = round * ((left * c + units - 1) / units) / c + left * c * part + 6.0;
+		if (time < least) {
+			least = time;
+			best = c;
+		}
+	}
+	return best;
+}
+
+static size_t ns_tiles(size_t p_rows, size_t q_rows, int tile, bool half) {
+	const size_t tp = p_rows / tile, tq = q_rows / tile;
+	return half ? tp * (tp + 1) / 2 : tp * tq;
+}
+
+// Bytes that the parts of a product's cut tiles take.
+static size_t ns_partial_bytes(size_t p_rows, size_t q_rows, int tile, bool half, uint32_t k_blocks, size_t batch) {
+	size_t left;
+	const unsigned cuts = ns_cuts(ns_tiles(p_rows, q_rows, tile, half), tile, k_blocks, batch, left);
+	return cuts > 1 ? left * cuts * tile * tile * sizeof(float) : 0;
+}
+
 template <int KIND>
 static int ns_product(const NsArgs& args, int tile, size_t p_rows, size_t q_rows, size_t batch) {
+	constexpr bool kHalf = KIND == kNsGram || KIND == kNsPoly;
 	NsArgs a = args;
 	a.tiles_p = (uint32_t)(p_rows / tile);
 	a.tiles_q = (uint32_t)(q_rows / tile);
-	const unsigned tiles = KIND == kNsGram || KIND == kNsPoly ? a.tiles_p * (a.tiles_p + 1) / 2 : a.tiles_p * a.tiles_q;
+	const unsigned tiles = (unsigned)ns_tiles(p_rows, q_rows, tile, kHalf);
+	size_t left = 0;
+	a.cuts = ns_cuts(tiles, tile, a.k_blocks, batch, left);
+	if (a.cuts == 1) left = 0;
+	a.whole = tiles - (unsigned)left;
 	a.band = (uint32_t)sqrt(tiles / 8.0);
 	if (a.band < 1) a.band = 1;
-	const dim3 grid(tiles, (unsigned)batch);
+	const dim3 grid(a.whole + (unsigned)left * a.cuts, (unsigned)batch);
 	hipStream_t stream = state().stream;
 	switch (tile) {
 		case 32: hipLaunchKernelGGL(ns_product_deep_kernel<KIND>, grid, dim3(kDeepWaves * 64), 0, stream, a); break;
@@ -795,6 +890,13 @@ static int ns_product(const NsArgs& args, int tile, size_t p_rows, size_t q_rows
 		default: hipLaunchKernelGGL((ns_product_kernel<256, 256, 2, 4, 1, 2, KIND>), grid, dim3(512), 0, stream, a); break;
 	}
 	TFHIP_CHECK_LAUNCH();
+	if (left) {
+		if (tile == 64)
+			hipLaunchKernelGGL((ns_join_kernel<64, 2, 2, KIND>), dim3((unsigned)left), dim3(256), 0, stream, a);
+		else
+			hipLaunchKernelGGL((ns_join_kernel<128, 2, 4, KIND>), dim3((unsigned)left * 4), dim3(256), 0, stream, a);
+		TFHIP_CHECK_LAUNCH();
+	}
 	return TFHIP_OK;
 }
 
@@ -838,7 +940,11 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 	const unsigned parts = (unsigned)(elements < 4096 ? 1 : elements / 4096 < 512 ? elements / 4096 : 512);
 	auto align = [](size_t b) { return (b + 255) & ~size_t(255); };
 	const size_t norm_bytes = align(batch * parts * sizeof(double)), x_bytes = align(batch * mp * np * 4), a_bytes = align(batch * mp * mp * 4);
-	char* base = (char*)scratch(norm_bytes + 4 * x_bytes + 2 * a_bytes);
+	const uint32_t blocks_m = (uint32_t)(mp / kNsStep), blocks_n = (uint32_t)(np / kNsStep);
+	const size_t parts_bytes[3] = {ns_partial_bytes(mp, mp, tile_half, true, blocks_n, batch), ns_partial_bytes(mp, mp, tile_half, true, blocks_m, batch),
+	                               ns_partial_bytes(mp, np, tile_full, false, blocks_m, batch)};
+	const size_t partial_bytes = std::max({parts_bytes[0], parts_bytes[1], parts_bytes[2]});
+	char* base = (char*)scratch(norm_bytes + 4 * x_bytes + 2 * a_bytes + partial_bytes);
 	if (!base) return TFHIP_ERR_HIP;
 	double* partial = (double*)base;
 	char* x = base + norm_bytes;
@@ -847,6 +953,7 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 	char* xt_next = x_next + x_bytes;
 	char* A = xt_next + x_bytes;
 	char* B = A + a_bytes;
+	float4* products_partial = (float4*)(B + a_bytes);
 
 	hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)batch * parts), dim3(256), 0, s.stream, g, partial, elements, parts, (elements & 3) == 0 && ((uintptr_t)g & 15) == 0);
 	TFHIP_CHECK_LAUNCH();
@@ -865,7 +972,8 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 		gram.straight_stride = gram.turned_stride = mp * 4;
 		gram.batch_p = gram.batch_q = mp * np * 4;
 		gram.batch_out = mp * mp * 4;
-		gram.k_blocks = (uint32_t)(np / kNsStep);
+		gram.partial = products_partial;
+		gram.k_blocks = blocks_n;
 		gram.alpha = (float)(scale_a / (scale_x * scale_x));
 		int rc = ns_product<kNsGram>(gram, tile_half, mp, mp, batch);
 		if (rc) return rc;
@@ -874,7 +982,7 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 		poly.straight = poly.turned = B;
 		poly.batch_p = poly.batch_q = poly.batch_addend = mp * mp * 4;
 		poly.addend_stride = mp * 4;
-		poly.k_blocks = (uint32_t)(mp / kNsStep);
+		poly.k_blocks = blocks_m;
 		poly.alpha = (float)(c * scale_b / (scale_a * scale_a));
 		poly.beta = (float)(b * scale_b / scale_a);
 		rc = ns_product<kNsPoly>(poly, tile_half, mp, mp, batch);
@@ -889,7 +997,8 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 		update.addend = turn ? x : xt;
 		update.addend_stride = (turn ? np : mp) * 4;
 		update.batch_addend = mp * np * 4;
-		update.k_blocks = (uint32_t)(mp / kNsStep);
+		update.partial = products_partial;
+		update.k_blocks = blocks_m;
 		if (last) {
 			update.out = out;
 			update.out_rows = rows;

@@ -198,3 +198,19 @@ def test_many_tiles(rt, batch, shape):
         # two steps: the first's error grows by at most 3.4445
         assert np.linalg.norm(got[k] - want) <= 3 * 3.5 * e(max(shape)) * np.linalg.norm(want)
     assert np.array_equal(run(rt, g, batch=batch, steps=steps), got)
+
+
+@pytest.mark.parametrize("shape", [(1300, 3400), (3400, 1300), (2000, 4100), (2990, 3000), (3500, 3500), (2040, 2010), (1500, 2960)])
+def test_products_whose_last_tiles_are_cut_along_k(rt, shape):
+    """More tiles of 64 or 128 than compute units: those left over are worked on in parts, whose sums meet in a fixed order."""
+    rng = np.random.default_rng(shape)
+    g = rng.standard_normal(shape, dtype=np.float32) + rng.standard_normal((shape[0], 4), dtype=np.float32) @ rng.standard_normal((4, shape[1]), dtype=np.float32)
+    got = run(rt, g, steps=2)
+    want = newton_schulz64(g, 2)
+    # two steps: the first's error grows by at most 3.4445
+    assert np.linalg.norm(got - want) <= 3 * 3.5 * e(max(shape)) * np.linalg.norm(want)
+    # no tile is off: every block of 32 x 32 by itself, against the size of a row and column of blocks
+    off = np.abs(got - want)
+    bound = 3 * 3.5 * e(max(shape)) * np.linalg.norm(want) / np.sqrt(want.size) * 64
+    assert off.max() <= bound
+    assert np.array_equal(run(rt, g, steps=2), got)
