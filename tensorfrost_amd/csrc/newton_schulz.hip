@@ -79,7 +79,8 @@ __device__ __forceinline__ void store_split_tile(const float (&v)[16], uint32_t*
 // ---- the norm and the first split -----------------------------------------------------------------
 
 // Partial sums of squares, in 64 bits: the square of a large fp32 number does not fit fp32. `vec`: every matrix starts on
-// 16 bytes and holds whole vectors. (4096 x 4096: 64 MiB.)
+// 16 bytes and holds whole vectors. (4096 x 4096, 64 MiB: 14 us, 4.7 TB/s; the split behind it, which writes both
+// orientations, 42 us.)
 __global__ __launch_bounds__(256) void ns_norm_kernel(const float* __restrict__ g, double* __restrict__ partial, size_t elements, unsigned parts, bool vec) {
 	__shared__ double red[4];
 	const size_t matrix = blockIdx.x / parts, part = blockIdx.x % parts;
@@ -272,7 +273,11 @@ __device__ __forceinline__ void finish_tile(const NsArgs& g, float (&v)[16], con
 	}
 }
 
-// A group of KS x WP x WQ waves owns a TP x TQ tile of the result. KS = 2: two sets of waves, each with one half of every step's
+// A group of KS x WP x WQ waves owns a TP x TQ tile of the result. Large products are bound by the matrix pipe and the clock that it
+// leaves: X of 4096 x 4096 350 us with tiles of 256 (1180 TFLOP/s of 16-bit products; 320 with everything but the matrix
+// instructions left out, 1.8 GHz; the library's product of 16-bit matrices of that size runs at 1330), A 195 and the join 6
+// (1060). Below about 2000 the way of a step through group memory and the barrier counts: A of 1003 x 1501 16 us, the pipe busy for 0.28 of
+// it. More stages change nothing there (3, 4 and 5: 15.8, 16.2 and 16.0), nor do fragments read one step ahead. KS = 2: two sets of waves, each with one half of every step's
 // columns, whose sums meet at the end. With one 32 x 32 tile per wave and as many groups as compute units that puts two
 // waves on a SIMD instead of one, and one reads while the other multiplies (A of 1003 x 1501: 18.2 -> 15.9 us).
 template <int TP, int TQ, int WP, int WQ, int KS, int STAGES, int KIND>
@@ -463,7 +468,8 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const NsArgs g) {
 // Few tiles: what counts is the way from the first load to the last store. A group of eight waves owns a 32 x 32 tile; each
 // wave multiplies the whole tile for 16 columns of every step of 128, and the waves' sums meet at the end. A wave fetches
 // the rows of one operand for one of a step's four blocks of columns; blocks beyond the end are skipped. (256 x 256, two
-// matrices: 5.3 us a product against 6.3 with 64 x 64 tiles and one wave per quarter; 64 x 64 tiles in this form: 7.4.)
+// matrices: 5.3 us a product, of which 3.5 are the launch, against 6.3 with 64 x 64 tiles and one wave per quarter. 64 x 64 tiles
+// in this form with four | eight waves: A of 1003 x 1501 22 | 16.4 us, X 20.5 | 24.4, where ns_product_kernel takes 15.8 and 19.2.)
 constexpr int kDeepWaves = 8, kDeepStages = 2;
 template <int KIND>
 __global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const NsArgs g) {
