@@ -128,6 +128,38 @@ def test_backward_against_float64(rt, shape):
     assert np.array_equal(xb.numpy(np.float32, shape), got) and np.array_equal(one_w.numpy(), dw.numpy()) and np.array_equal(one_b.numpy(), db.numpy())
 
 
+# on both sides of the number of rows up to which one launch does everything, unless dx takes the place of an input
+@pytest.mark.parametrize("rows", [1, 15, 511, 512, 513])
+@pytest.mark.parametrize("cols", [1, 17, 250, 1024, 1030, 9000])
+def test_few_rows_backward_in_place_and_not(rt, rows, cols):
+    x, w, _, dy = make(rows, cols, seed=3)
+    xb, wb = rt.DeviceBuffer.from_numpy(x), rt.DeviceBuffer.from_numpy(w)
+    mean, rstd = rt.DeviceBuffer(rows), rt.DeviceBuffer(rows)
+    rt.layer_norm_rows(xb, wb, None, rt.DeviceBuffer(x.size), rows, cols, mean=mean, rstd=rstd)
+    m, s = mean.numpy().astype(np.float64)[:, None], rstd.numpy().astype(np.float64)[:, None]
+    terms = dy * ((x - m) * s)
+    chain = (rows + 8) * U  # a sum of `rows` terms in any order, each off by a few roundings
+    results = []
+    for place in ("own", "dy", "x"):
+        xb, dyb = rt.DeviceBuffer.from_numpy(x), rt.DeviceBuffer.from_numpy(dy)
+        dx = {"own": guarded(rt, x.size), "dy": dyb, "x": xb}[place]
+        dw, db = guarded(rt, cols), guarded(rt, cols)
+        rt.layer_norm_rows_backward(xb, dyb, wb, mean, rstd, rows, cols, dx=dx, dweight=dw, dbias=db)
+        assert (np.abs(dw.numpy() - terms.sum(0)) <= chain * np.abs(terms).sum(0) + 4 * U * (np.abs(dy) * s * (np.abs(x) + np.abs(m))).sum(0)).all()
+        assert (np.abs(db.numpy() - dy.astype(np.float64).sum(0)) <= chain * np.abs(dy).sum(0)).all()
+        assert untouched(dw) and untouched(db) and (place != "own" or untouched(dx))
+        results.append(dx.numpy(np.float32, x.shape))
+    assert np.array_equal(results[0], results[1]) and np.array_equal(results[0], results[2])
+    # each gradient by itself: the same words as together
+    for name in ("dx", "dweight", "dbias"):
+        n = x.size if name == "dx" else cols
+        alone, together = guarded(rt, n), {k: rt.DeviceBuffer(x.size if k == "dx" else cols) for k in ("dx", "dweight", "dbias")}
+        xb, dyb = rt.DeviceBuffer.from_numpy(x), rt.DeviceBuffer.from_numpy(dy)
+        rt.layer_norm_rows_backward(xb, dyb, wb, mean, rstd, rows, cols, **{name: alone})
+        rt.layer_norm_rows_backward(xb, dyb, wb, mean, rstd, rows, cols, **together)
+        assert untouched(alone) and np.array_equal(alone.numpy(np.uint32), together[name].numpy(np.uint32))
+
+
 # rows that end one, two and three elements into a vector, on both sides of the widths at which another kernel takes over
 @pytest.mark.parametrize("cols", [1023, 1025, 2047, 2049, 4093, 4095, 4097, 4098, 4099, 8190, 8193, 8195, 16381, 16382, 16383, 16385, 16386, 24577, 24579])
 @pytest.mark.parametrize("rows", [1, 7])
