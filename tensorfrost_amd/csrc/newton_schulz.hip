@@ -468,7 +468,8 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const NsArgs g) {
 // Few tiles: what counts is the way from the first load to the last store. A group of eight waves owns a 32 x 32 tile; each
 // wave multiplies the whole tile for 16 columns of every step of 128, and the waves' sums meet at the end. A wave fetches
 // the rows of one operand for one of a step's four blocks of columns; blocks beyond the end are skipped. (256 x 256, two
-// matrices: 5.3 us a product, of which 3.5 are the launch, against 6.3 with 64 x 64 tiles and one wave per quarter. 64 x 64 tiles
+// matrices: 5.1 us a product, about half of it the launch's own, against 6.3 with 64 x 64 tiles and one wave per quarter; with one step
+// asked for ahead instead of two 5.3, at 512 x 512 7.0 against 6.5. 64 x 64 tiles
 // in this form with four | eight waves: A of 1003 x 1501 22 | 16.4 us, X 20.5 | 24.4, where ns_product_kernel takes 15.8 and 19.2.)
 constexpr int kDeepWaves = 8, kDeepStages = 2;
 template <int KIND>
@@ -493,19 +494,21 @@ __global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const 
 	const uint32_t lds0 = lds_offset(lds) + block * kPanel + (wave & 1) * T * kNsBlock;
 
 	const uint32_t steps = (g.k_blocks + kBlocks - 1) / kBlocks;
-	uint32_t fetched = 0, fill = 0;
-	auto fetch = [&]() {
-		if (fetched * kBlocks + block < g.k_blocks) {
+	auto mine = [&](uint32_t step) { return step * kBlocks + block < g.k_blocks; };  // whether this wave has a part in a step
+	uint32_t fill = 0;
+	auto fetch = [&](uint32_t step) {
+		if (mine(step)) {
 #pragma unroll
 			for (int i = 0; i < kLoads; i++) load_to_lds(lds0 + fill + i * 1024, offset[i], src);
 		}
 		src += kBlocks * kNsBlock;
-		fetched++;
-		fill = fill + kStage == kDeepStages * kStage ? 0 : fill + kStage;
+		fill = kStage - fill;
 	};
-	fetch();
+	// Older than the panels' loads, so that the counter that is waited for says nothing of it; it arrives while the products run.
 	Addend addend;
-	if (KIND != kNsGram && wave == 0) load_addend(g, addend, tp * T, tq * T);  // arrives while the products run
+	if (KIND != kNsGram && wave == 0) load_addend(g, addend, tp * T, tq * T);
+	fetch(0);
+	fetch(1);
 
 	floatx16 acc;
 #pragma unroll
@@ -515,15 +518,21 @@ __global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const 
 	const char* frag_q = frag_p + T * kNsBlock;
 	uint32_t cur = 0;
 	for (uint32_t k = 0; k < steps; k++) {
-		wait_loads<0>();
-		__syncthreads();  // everybody's part of this step is there, and everybody has read the step before
-		if (fetched < steps) fetch();
-		if (k * kBlocks + block < g.k_blocks) {
+		if (mine(k + 1))
+			wait_loads<kLoads>();
+		else
+			wait_loads<0>();
+		__syncthreads();  // everybody's part of this step is there
+		if (mine(k)) {
 			const half8 p_hi = *reinterpret_cast<const half8*>(frag_p + cur + hi_at), p_lo = *reinterpret_cast<const half8*>(frag_p + cur + lo_at);
 			const half8 q_hi = *reinterpret_cast<const half8*>(frag_q + cur + hi_at), q_lo = *reinterpret_cast<const half8*>(frag_q + cur + lo_at);
 			acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_lo, q_hi, acc, 0, 0, 0);
 			acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi, q_lo, acc, 0, 0, 0);
 			acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(p_hi, q_hi, acc, 0, 0, 0);
+		}
+		if (k + 2 < steps) {
+			__syncthreads();  // everybody has read this step: its panels' memory takes the step after the next
+			fetch(k + 2);
 		}
 		cur = kStage - cur;
 	}
