@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void embedding_kernel(const int32_t* __restric
 // Up to kAllPairs positions by counting: the place of position i is the number of keys that are smaller, or equal and
 // earlier. A key is the token read as unsigned: what names no row (negative, or beyond the table) is at least vocab and comes
 // last. A group places 64 positions, one per lane of each of its waves; the waves each compare them with their share of
-// the keys: a lane broadcast, a compare and an add per pair. 500 positions 4.7 us, 4096 9 to 11, 8192 16 (the kernels below: 4096 15,
+// the keys: a lane broadcast, a compare and an add per pair. 2049 positions 7 us, 4096 9 to 11, 8192 16 (the kernels below: 4096 15,
 // 8192 16).
 constexpr uint32_t kAllPairs = 4096;
 constexpr int kCountWaves = 16;
@@ -408,80 +408,101 @@ static int embedding_sums(const uint32_t* keys, const uint32_t* order, const flo
 
 // ---- few positions ----------------------------------------------------------------------------------------
 
-// Up to kFewPositions positions of a table of moderate size in one launch, without an order of all of them: a group owns
-// kFewRows rows of the table, looks through all tokens (one per thread), lists the positions of its rows in their order (8 waves, a ballot
-// each) and adds up the rows' dy. A wave takes a row with few positions; a row with more than kFewAlone is cut into eight
-// parts of neighbouring positions, one per wave, added in their order at the end. Rows without positions get their zeros on
-// the way. Against the three launches below (counting, sums, joins; us in the kernels): 500 x 250 over 1009 rows 8.0 | 14.0,
-// 512 x 512 over 8192 12.2 | 16.0, all 512 positions one token 13.8 | 13.3. With more tokens, columns or rows of the table the
-// looking through and the long rows cost more than the launches: 1000 x 1024 over 32768 46 | 37, over one row 134 | 15.
-constexpr uint32_t kFewPositions = 512;
-constexpr size_t kFewVocab = 8192, kFewCols = 512;
-constexpr int kFewRows = 8, kFewWaves = 8, kFewAlone = 32;
-static_assert(kFewWaves * 64 == kFewPositions, "a thread per position");
+// Up to kFewPositions positions in one launch, without an order of all of them. A group owns some rows of the table, the 64 VEC
+// columns of a wave of them: it counts the positions of each, with the tokens in group memory, writes zeros into the rows
+// without any as one stretch of memory, and adds up the others. A wave takes a row with few positions, which it finds in
+// their order by a ballot for every 64 tokens; a row with more than kFewAlone is cut into eight parts of neighbouring positions, one
+// per wave, added in their order at the end. us in the kernels, this one | the three launches below, which also wait for each
+// other for 6 us in all: 500 x 250 over 1009 rows 5.8 | 14.0, 37 x 560 over 22709 11 | 21, 1000 x 1024 over 100 9.0 | 14.6, 1551 x 86
+// over 6876 8.7 | 15.8, 2048 x 256 over 50000 13.6 | 24.9; the frequent rows decide where it ends: 2048 x 64 over 50 rows 22 | 16,
+// 2048 x 1024 over one 25 | 19, and 4096 x 100 over 100 34 | 20.
+constexpr uint32_t kFewPositions = 2048, kFewMostRows = 256;
+constexpr int kFewWaves = 8, kFewThreads = kFewWaves * 64, kFewAlone = 32;
+constexpr size_t kFewVocab = (size_t)1 << 30, kFewCols = 65535 * 64;  // a launch has fewer than 2^32 threads
 
 template <int VEC>
-__global__ __launch_bounds__(kFewWaves * 64) void embedding_few_kernel(const int32_t* __restrict__ tokens, const float* __restrict__ dy, float* __restrict__ dtable, uint32_t n, uint32_t vocab,
-                                                                       size_t cols, float scale) {
+__global__ __launch_bounds__(kFewThreads) void embedding_few_kernel(const int32_t* __restrict__ tokens, const float* __restrict__ dy, float* __restrict__ dtable, uint32_t n, uint32_t vocab,
+                                                                    size_t cols, float scale, uint32_t rows_of_group) {
 	typedef typename Floats<VEC>::type Vec;
-	__shared__ uint16_t list[kFewRows][kFewPositions];
-	__shared__ uint32_t found[kFewRows][kFewWaves];
+	__shared__ uint32_t token[kFewPositions];
+	__shared__ uint32_t count[kFewMostRows];
+	__shared__ uint16_t list[kFewWaves][kFewAlone], long_list[kFewPositions];
 	__shared__ Vec parts[kFewWaves][64];
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	const uint32_t v0 = blockIdx.x * kFewRows;
-	const uint32_t token = threadIdx.x < n ? (uint32_t)tokens[threadIdx.x] : 0xFFFFFFFFu;  // names no row
-	const uint32_t mine = token < vocab ? token - v0 : 0xFFFFFFFFu;                         // its row of this group's, if below kFewRows
-	uint64_t votes[kFewRows];
-	uint32_t count[kFewRows];  // the same in every thread
-#pragma unroll
-	for (int r = 0; r < kFewRows; r++) {
-		votes[r] = __ballot(mine == (uint32_t)r);
-		if (lane == 0) found[r][wave] = __popcll(votes[r]);
-	}
+	const uint32_t v0 = blockIdx.x * rows_of_group, rows = vocab - v0 < rows_of_group ? vocab - v0 : rows_of_group;
+	const size_t c = (size_t)blockIdx.y * 64 * VEC + (size_t)lane * VEC;  // this lane's columns
+	const bool inside = c < cols;
+	const uint32_t chunks = (n + 63) / 64;
+	for (uint32_t r = threadIdx.x; r < kFewMostRows; r += kFewThreads) count[r] = 0;
 	__syncthreads();
 #pragma unroll
-	for (int r = 0; r < kFewRows; r++) {
-		uint32_t at = 0;
-		count[r] = 0;
+	for (uint32_t j = 0; j < kFewPositions / kFewThreads; j++) {
+		const uint32_t i = j * kFewThreads + threadIdx.x;
+		const uint32_t t = i < n ? (uint32_t)tokens[i] : 0xFFFFFFFFu;  // which names no row
+		token[i] = t;
+		if (t - v0 < rows) atomicAdd(&count[t - v0], 1u);
+	}
+	__syncthreads();
+	const size_t c0 = (size_t)blockIdx.y * 64 * VEC;
+	const uint32_t width = (uint32_t)(cols - c0 < 64 * VEC ? (cols - c0) / VEC : 64);
+	for (uint32_t i = threadIdx.x; i < rows * width; i += kFewThreads) {
+		const uint32_t r = i / width;
+		if (count[r] == 0) __builtin_nontemporal_store(Vec(0.0f), reinterpret_cast<Vec*>(dtable + (size_t)(v0 + r) * cols + c0 + (i - r * width) * VEC));
+	}
+	// the sum of the rows of dy that `from` lists in [first, last)
+	auto add_up = [&](const uint16_t* from, uint32_t first, uint32_t last) {
+		Vec sum = Vec(0.0f);
+		if (!inside) return sum;
+		for (uint32_t p0 = first; p0 < last; p0 += kSumRows) {
+			Vec v[kSumRows];
 #pragma unroll
-		for (int w = 0; w < kFewWaves; w++) {
-			const uint32_t f = found[r][w];
-			at += w < wave ? f : 0;
-			count[r] += f;
+			for (int u = 0; u < kSumRows; u++) v[u] = *reinterpret_cast<const Vec*>(dy + (size_t)from[p0 + u < last ? p0 + u : p0] * cols + c);
+#pragma unroll
+			for (int u = 0; u < kSumRows; u++)
+				if (p0 + u < last) sum += v[u];
 		}
-		if (mine == (uint32_t)r) list[r][at + __popcll(votes[r] & ((1ull << lane) - 1))] = (uint16_t)threadIdx.x;
-	}
-	__syncthreads();
-#pragma unroll
-	for (int r = 0; r < kFewRows; r++) {
-		if (v0 + r >= vocab) break;
-		const bool shared = count[r] > kFewAlone;
-		if (!shared && r % kFewWaves != wave) continue;
-		// this wave's positions of the row
-		const uint32_t share = (count[r] + kFewWaves - 1) / kFewWaves;
-		const uint32_t first = shared ? wave * share : 0, last = shared ? (first + share < count[r] ? first + share : count[r]) : count[r];
-		for (size_t c0 = 0; c0 < cols; c0 += 64 * VEC) {
-			const size_t c = c0 + (size_t)lane * VEC;
-			Vec sum = Vec(0.0f);
-			if (c < cols)
-				for (uint32_t p0 = first; p0 < last; p0 += kSumRows) {
-					Vec v[kSumRows];
-#pragma unroll
-					for (int u = 0; u < kSumRows; u++) v[u] = *reinterpret_cast<const Vec*>(dy + (size_t)list[r][p0 + u < last ? p0 + u : p0] * cols + c);
-#pragma unroll
-					for (int u = 0; u < kSumRows; u++)
-						if (p0 + u < last) sum += v[u];
-				}
-			if (shared) {
-				parts[wave][lane] = sum;
-				__syncthreads();
-				if (wave == 0) {
-#pragma unroll
-					for (int w = 1; w < kFewWaves; w++) sum += parts[w][lane];
-				}
+		return sum;
+	};
+	uint32_t turn = 0;  // rows with few positions go to the waves in turn
+	for (uint32_t r0 = 0; r0 < rows; r0 += 64) {
+		const uint32_t of_lane = count[r0 + lane];
+		uint64_t few = __ballot(of_lane > 0 && of_lane <= kFewAlone);
+		for (; few; few &= few - 1) {
+			if (turn++ % kFewWaves != (uint32_t)wave) continue;
+			const uint32_t r = r0 + __builtin_ctzll(few), found = count[r];
+			uint32_t at = 0;
+			for (uint32_t k = 0; k < chunks; k++) {
+				const uint64_t same = __ballot(token[k * 64 + lane] == v0 + r);
+				if ((same >> lane) & 1) list[wave][at + __popcll(same & ((1ull << lane) - 1))] = (uint16_t)(k * 64 + lane);
+				at += __popcll(same);
 			}
-			if ((!shared || wave == 0) && c < cols) __builtin_nontemporal_store(sum * scale, reinterpret_cast<Vec*>(dtable + (size_t)(v0 + r) * cols + c));
-			if (shared) __syncthreads();
+			__builtin_amdgcn_wave_barrier();
+			const Vec sum = add_up(list[wave], 0, found);
+			if (inside) __builtin_nontemporal_store(sum * scale, reinterpret_cast<Vec*>(dtable + (size_t)(v0 + r) * cols + c));
+			__builtin_amdgcn_wave_barrier();
+		}
+	}
+	for (uint32_t r0 = 0; r0 < rows; r0 += 64) {
+		const uint32_t of_lane = count[r0 + lane];
+		for (uint64_t many = __ballot(of_lane > kFewAlone); many; many &= many - 1) {  // the same in every wave
+			const uint32_t r = r0 + __builtin_ctzll(many), found = count[r];
+			uint32_t at = 0;
+			for (uint32_t k = 0; k < chunks; k++) {
+				const uint64_t same = __ballot(token[k * 64 + lane] == v0 + r);
+				if (k % kFewWaves == (uint32_t)wave && ((same >> lane) & 1)) long_list[at + __popcll(same & ((1ull << lane) - 1))] = (uint16_t)(k * 64 + lane);
+				at += __popcll(same);
+			}
+			__syncthreads();
+			const uint32_t share = (found + kFewWaves - 1) / kFewWaves, first = wave * share < found ? wave * share : found, last = first + share < found ? first + share : found;
+			Vec sum = add_up(long_list, first, last);
+			parts[wave][lane] = sum;
+			__syncthreads();
+			if (wave == 0 && inside) {
+#pragma unroll
+				for (int w = 1; w < kFewWaves; w++) sum += parts[w][lane];
+				__builtin_nontemporal_store(sum * scale, reinterpret_cast<Vec*>(dtable + (size_t)(v0 + r) * cols + c));
+			}
+			__syncthreads();
 		}
 	}
 }
@@ -532,11 +553,14 @@ extern "C" int tfhip_embedding_rows_backward_f32(const int32_t* tokens, const fl
 	if (n == 0) return tfhip_fill_u32(dtable, 0u, vocab * cols);
 	if (n <= kFewPositions && vocab <= kFewVocab && cols <= kFewCols) {
 		const RowShape r = row_shape(cols, dy, dtable);
-		const dim3 grid((unsigned)((vocab + kFewRows - 1) / kFewRows)), block(kFewWaves * 64);
+		// four groups a unit, with 8 to kFewMostRows rows each
+		const size_t stretches = (cols + 64 * r.vec - 1) / (64 * r.vec), wanted = (vocab * stretches + s.compute_units * 4 - 1) / (s.compute_units * 4);
+		const size_t rows = wanted < 8 ? 8 : wanted < kFewMostRows ? wanted : kFewMostRows;
+		const dim3 grid((unsigned)((vocab + rows - 1) / rows), (unsigned)stretches), block(kFewThreads);
 		switch (r.vec) {
-			case 4: hipLaunchKernelGGL(embedding_few_kernel<4>, grid, block, 0, s.stream, tokens, dy, dtable, (uint32_t)n, (uint32_t)vocab, cols, scale); break;
-			case 2: hipLaunchKernelGGL(embedding_few_kernel<2>, grid, block, 0, s.stream, tokens, dy, dtable, (uint32_t)n, (uint32_t)vocab, cols, scale); break;
-			default: hipLaunchKernelGGL(embedding_few_kernel<1>, grid, block, 0, s.stream, tokens, dy, dtable, (uint32_t)n, (uint32_t)vocab, cols, scale); break;
+			case 4: hipLaunchKernelGGL(embedding_few_kernel<4>, grid, block, 0, s.stream, tokens, dy, dtable, (uint32_t)n, (uint32_t)vocab, cols, scale, (uint32_t)rows); break;
+			case 2: hipLaunchKernelGGL(embedding_few_kernel<2>, grid, block, 0, s.stream, tokens, dy, dtable, (uint32_t)n, (uint32_t)vocab, cols, scale, (uint32_t)rows); break;
+			default: hipLaunchKernelGGL(embedding_few_kernel<1>, grid, block, 0, s.stream, tokens, dy, dtable, (uint32_t)n, (uint32_t)vocab, cols, scale, (uint32_t)rows); break;
 		}
 		TFHIP_CHECK_LAUNCH();
 		return TFHIP_OK;
@@ -544,8 +568,8 @@ extern "C" int tfhip_embedding_rows_backward_f32(const int32_t* tokens, const fl
 	const bool radix = n > kMostTiled;
 	int digits = 1;  // of keys 0 .. vocab
 	while (digits < 4 && vocab >> (8 * digits)) digits++;
-	// Rows a wave adds up one after the other: few rows need shorter chains, more of them at once (500 x 250: sums and
-	// joins of a larger table 9.6 us with 16, 11.3 with 32, 16.5 with 64), many rows fewer parts to join (65536 x 1024: 93, 89 and 88.5 us).
+	// Rows a wave adds up one after the other: few rows need shorter chains, more of them at once (sums and joins, us, with 16 | 32:
+	// 4096 x 512 9.6 | 11.7, 8192 x 64 10.2 | 12.1), many rows fewer parts to join (65536 x 1024 93 | 89, with 64 88.5).
 	uint32_t segment = n * cols >= (size_t)1 << 22 ? 32 : 16;
 	while (n / segment >= (size_t)1 << 22) segment *= 2;  // a launch has fewer than 2^32 threads
 	const size_t segments = (n + segment - 1) / segment;

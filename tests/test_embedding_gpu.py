@@ -124,6 +124,24 @@ def test_nan_and_infinity_reach_only_the_rows_that_hold_them(rt):
     assert (~np.isfinite(got)).sum() == 1
 
 
+@pytest.mark.parametrize("shape", [(2047, 300, 20), (2048, 8193, 257), (2048, 7, 1030), (2049, 8193, 64), (2048, 70001, 3), (1, 300000, 5), (40, 1100000, 2), (2000, 1025, 65), (33, 1, 600), (1024, 257, 256)])
+@pytest.mark.parametrize("kind", ["skewed", "one token", "runs of 32 and 33", "the last rows", "none"])
+def test_gradient_of_few_positions(rt, shape, kind):
+    """One launch up to 2048 positions: groups of 8 to 256 rows, rows with up to 32 positions and with more."""
+    n, vocab, cols = shape
+    rng = np.random.default_rng([n, vocab, cols, 2])
+    t = {"skewed": lambda: tokens_for(n, vocab, 7, pad=0.1), "one token": lambda: np.full(n, vocab - 1, np.int32), "runs of 32 and 33": lambda: (np.repeat(np.arange(n), 1 + 31 + np.arange(n) % 2)[:n] % vocab).astype(np.int32),
+         "the last rows": lambda: (vocab - 1 - rng.integers(0, min(vocab, 40), n)).astype(np.int32), "none": lambda: np.where(np.arange(n) % 2, np.iinfo(np.int32).min, np.iinfo(np.int32).max).astype(np.int32)}[kind]()
+    dy = rng.integers(-4, 5, (n, cols)).astype(np.float32)
+    dy[(t < 0) | (t >= vocab)] = np.nan  # nobody's
+    d = rt.DeviceBuffer(vocab * cols + 64)
+    d.fill(0x7FC00000)
+    rt.embedding_rows_backward(rt.DeviceBuffer.from_numpy(t), rt.DeviceBuffer.from_numpy(dy), d, n, vocab, cols, scale=2.0)
+    got = d.numpy(np.float32)
+    assert np.array_equal(got[: vocab * cols].reshape(vocab, cols), (2.0 * gradient(t, dy, vocab)).astype(np.float32))
+    assert np.isnan(got[vocab * cols:]).all()
+
+
 # on both sides of the sizes at which another kernel takes over: 512 positions, 8192 rows, 512 columns, 4096 and 131072 positions
 @pytest.mark.parametrize("shape", [(511, 8191, 511), (512, 8192, 512), (512, 8193, 512), (513, 8192, 64), (512, 9, 513), (512, 7, 512), (65, 8, 130), (4095, 300, 20), (4096, 300, 20), (4097, 300, 20),
                                    (131072, 300, 4), (131073, 300, 4)])
