@@ -274,22 +274,22 @@ __global__ __launch_bounds__(kLnThreads) void layer_norm_apply_kernel(const floa
 
 // ---- backward --------------------------------------------------------------------------------------
 
-// dw and db of kLnColumns columns from c0 on, by one block that goes through all rows: with few rows. kLnColumns threads side by
-// side, the others at other rows; the threads' sums are added in a fixed order.
+// dw and db of some columns (a power of two up to kLnColumns) from c0 on, by one block that goes through all rows: with few
+// rows. That many threads side by side, the others at other rows; the threads' sums are added in a fixed order.
 constexpr int kLnColumns = 16;
 template <int THREADS>
 __device__ __forceinline__ void column_sums(const float* x, const float* dy, const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ dweight, float* __restrict__ dbias,
-                                            size_t rows, int cols, int c0) {
+                                            size_t rows, int cols, int c0, int columns) {
 	__shared__ float red[2][THREADS / 64][kLnColumns];
-	constexpr int kSlices = THREADS / kLnColumns, kAhead = 8;
-	const int c = c0 + threadIdx.x % kLnColumns;
+	constexpr int kAhead = 8;
+	const int slices = THREADS / columns, mine = threadIdx.x & (columns - 1), c = c0 + mine;
 	float dw = 0.0f, db = 0.0f;
 	if (c < cols)
-		for (size_t r0 = threadIdx.x / kLnColumns; r0 < rows; r0 += kSlices * kAhead) {
+		for (size_t r0 = threadIdx.x / columns; r0 < rows; r0 += slices * kAhead) {
 			float vx[kAhead], vdy[kAhead], m[kAhead], s[kAhead];
 #pragma unroll
 			for (int u = 0; u < kAhead; u++) {
-				const size_t r = r0 + u * kSlices < rows ? r0 + u * kSlices : r0;
+				const size_t r = r0 + u * slices < rows ? r0 + u * slices : r0;
 				vx[u] = x[r * cols + c];
 				vdy[u] = dy[r * cols + c];
 				m[u] = mean[r];
@@ -297,27 +297,26 @@ __device__ __forceinline__ void column_sums(const float* x, const float* dy, con
 			}
 #pragma unroll
 			for (int u = 0; u < kAhead; u++) {
-				if (r0 + u * kSlices >= rows) break;
+				if (r0 + u * slices >= rows) break;
 				dw += vdy[u] * ((vx[u] - m[u]) * s[u]);
 				db += vdy[u];
 			}
 		}
-#pragma unroll
-	for (int off = kLnColumns; off < 64; off *= 2) {
+	for (int off = columns; off < 64; off *= 2) {
 		dw += __shfl_xor(dw, off, 64);
 		db += __shfl_xor(db, off, 64);
 	}
 	const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-	if (lane < kLnColumns) {
+	if (lane < columns) {
 		red[0][wave][lane] = dw;
 		red[1][wave][lane] = db;
 	}
 	__syncthreads();
-	if (threadIdx.x < 2 * kLnColumns) {
-		const int which = threadIdx.x / kLnColumns;
+	if ((int)threadIdx.x < 2 * columns) {
+		const int which = (int)threadIdx.x >= columns;
 		float t = 0.0f;
 #pragma unroll
-		for (int w = 0; w < THREADS / 64; w++) t += red[which][w][threadIdx.x % kLnColumns];
+		for (int w = 0; w < THREADS / 64; w++) t += red[which][w][mine];
 		float* to = which ? dbias : dweight;
 		if (to && c < cols) to[c] = t;
 	}
@@ -331,10 +330,10 @@ __device__ __forceinline__ void column_sums(const float* x, const float* dy, con
 template <int GROUP, int E, Access ACCESS, int R>
 __global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void layer_norm_backward_kernel(const float* x, const float* dy, const float* __restrict__ weight, const float* __restrict__ mean,
                                                                                         const float* __restrict__ rstd, float* dx, float* __restrict__ partial, size_t rows, int cols,
-                                                                                        unsigned row_blocks, float* __restrict__ dweight, float* __restrict__ dbias) {
+                                                                                        unsigned row_blocks, int columns, float* __restrict__ dweight, float* __restrict__ dbias) {
 	constexpr int kThreads = GROUP > 256 ? GROUP : 256, kGroups = kThreads / GROUP;
 	if (blockIdx.x >= row_blocks) {
-		column_sums<kThreads>(x, dy, mean, rstd, dweight, dbias, rows, cols, (blockIdx.x - row_blocks) * kLnColumns);
+		column_sums<kThreads>(x, dy, mean, rstd, dweight, dbias, rows, cols, (blockIdx.x - row_blocks) * columns, columns);
 		return;
 	}
 	// for the sums of a large group (two in turn, so that one barrier a row is enough), then for the join of the groups' columns
@@ -522,10 +521,11 @@ __global__ __launch_bounds__(kFoldWaves * 64) void layer_norm_fold_kernel(const 
 // A row of 16384 in registers takes 100 us forward and 151 backward for 4096 rows, one of 16388 in segments 121 and 335.
 constexpr size_t kLnMostInRegisters = 16384;
 
-// Up to so many rows the backward pass is one launch: dw and db need only the rows' statistics, which are inputs, so other
-// blocks of the same launch sum the columns, and x and dy are read twice; where dx is x or dy, in a launch before. us in
-// the kernels, one launch | two, which also wait 3.5 us for each other: 16 x 1024 3.3 | 7.0, 256 x 1024 4.8 | 8.0, 256 x 4096 5.2 |
-// 10.7, 512 x 256 6.8 | 7.0, 512 x 4096 13.5 | 17.0, 1037 x 772 22.8 | 8.7.
+// Up to so many rows (twice as many narrow ones) the backward pass is one launch: dw and db need only the rows' statistics, which
+// are inputs, so other blocks of the same launch sum the columns, and x and dy are read twice; where dx is x or dy, in a launch
+// before. us in the kernels, one launch | two, which also wait 3 us for each other: 16 x 1024 3.3 | 7.0, 256 x 1024 4.8 | 8.0, 256 x
+// 4096 5 | 10.7, 512 x 256 4.0 | 7.0, 512 x 4096 13.5 | 17.0, 1024 x 64 5.0 | 6.1; beyond, 1037 x 772 11.6 | 8.7, 2048 x 256 11.6 | 7.0.
+constexpr size_t kLnNarrow = 256;
 constexpr size_t kLnFewRows = 512;
 
 // Calls f with (threads of a row, elements of a thread, rows at a time) as constants: the smallest group that holds the
@@ -583,15 +583,18 @@ static int layer_norm_backward(const float* x, const float* dy, const float* wei
 		constexpr int kGroup = decltype(group)::value, kThreads = kGroup > 256 ? kGroup : 256, kRows = kThreads / kGroup * decltype(r)::value;
 		// as many blocks as stay resident, 1024 threads a unit
 		const size_t most = (size_t)s.compute_units * 1024 / kThreads, want = (rows + kRows - 1) / kRows, blocks = want < most ? want : most;
+		// narrow stretches of columns, so that a thread has fewer rows, where the matrix is small enough to be read in such pieces
+		// (16 | 4 columns: 512 x 256 6.8 | 4.0 us, 512 x 1024 7.1 | 5.8, 512 x 4096 13 | 26)
+		const int columns = rows > 128 && cols <= 1024 ? 4 : kLnColumns;
 		auto launch = [&](unsigned row_blocks, unsigned column_blocks, float* partial) {
 			if (rc || row_blocks + column_blocks == 0) return;
 			hipLaunchKernelGGL((layer_norm_backward_kernel<kGroup, decltype(e)::value, decltype(access)::value, decltype(r)::value>), dim3(row_blocks + column_blocks), dim3(kThreads), 0, s.stream, x,
-			                   dy, weight, mean, rstd, dx, partial, rows, (int)cols, row_blocks, dweight, dbias);
+			                   dy, weight, mean, rstd, dx, partial, rows, (int)cols, row_blocks, columns, dweight, dbias);
 			const hipError_t err = hipGetLastError();
 			if (err != hipSuccess) rc = fail_hip(err, "layer norm backward launch");
 		};
-		if (rows <= kLnFewRows) {
-			const unsigned row_blocks = dx ? (unsigned)blocks : 0, column_blocks = dweight || dbias ? (unsigned)((cols + kLnColumns - 1) / kLnColumns) : 0;
+		if (rows <= (cols <= kLnNarrow ? 2 * kLnFewRows : kLnFewRows)) {
+			const unsigned row_blocks = dx ? (unsigned)blocks : 0, column_blocks = dweight || dbias ? (unsigned)((cols + columns - 1) / columns) : 0;
 			if (dx == x || dx == dy) {  // all columns before the first row is overwritten
 				launch(0, column_blocks, nullptr);
 				launch(row_blocks, 0, nullptr);

@@ -129,8 +129,8 @@ def test_backward_against_float64(rt, shape):
 
 
 # on both sides of the number of rows up to which one launch does everything, unless dx takes the place of an input
-@pytest.mark.parametrize("rows", [1, 15, 511, 512, 513])
-@pytest.mark.parametrize("cols", [1, 17, 250, 1024, 1030, 9000])
+@pytest.mark.parametrize("rows", [1, 15, 128, 129, 511, 512, 513, 1024, 1025])
+@pytest.mark.parametrize("cols", [1, 17, 250, 256, 257, 1024, 1030, 9000])
 def test_few_rows_backward_in_place_and_not(rt, rows, cols):
     x, w, _, dy = make(rows, cols, seed=3)
     xb, wb = rt.DeviceBuffer.from_numpy(x), rt.DeviceBuffer.from_numpy(w)
