@@ -307,9 +307,12 @@ def sgemm(layout: str, a: DeviceBuffer, b: DeviceBuffer, c: DeviceBuffer, m: int
 
 
 def _words(buf: DeviceView | None, n_words: int, name: str):
-    """The address of a buffer that has to hold at least n_words; None stays None."""
+    """The address of a buffer that has to hold at least n_words; None stays None. A buffer that was freed is an error, not None:
+    the calls read a null pointer as one that was not given."""
     if buf is None:
         return None
+    if buf.ptr is None:
+        raise ValueError(f"{name} has been freed")
     if buf.n_words < n_words:
         raise ValueError(f"{name} holds {buf.n_words} words, {n_words} are needed")
     return buf.ptr

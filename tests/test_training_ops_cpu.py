@@ -126,3 +126,23 @@ def test_views_own_nothing():
             runtime.DeviceBuffer.view(bad, 4)
     with pytest.raises(ValueError):
         runtime.DeviceBuffer.view(BASE, 0)
+
+
+def test_freed_buffers_are_refused_not_taken_as_left_out():
+    """A null pointer means "not given" to the library: no weight, no bias, an output that is not wanted."""
+    def gone():
+        v = buf(1000)
+        v.free()
+        return v
+
+    big = buf(1000)
+    forward = lambda **kw: runtime.layer_norm_rows(**{**dict(x=big, weight=big, bias=big, y=big, rows=8, cols=16), **kw})  # noqa: E731
+    backward = lambda **kw: runtime.layer_norm_rows_backward(**{**dict(x=big, dy=big, weight=big, mean=big, rstd=big, rows=8, cols=16, dx=big), **kw})  # noqa: E731
+    lookup = lambda **kw: runtime.embedding_rows(**{**dict(tokens=big, table=big, out=big, n=8, vocab=5, cols=16), **kw})  # noqa: E731
+    gradient = lambda **kw: runtime.embedding_rows_backward(**{**dict(tokens=big, dy=big, dtable=big, n=8, vocab=5, cols=16), **kw})  # noqa: E731
+    schulz = lambda **kw: runtime.newton_schulz(**{**dict(g=big, out=big, rows=8, cols=16), **kw})  # noqa: E731
+    for f, names in ((forward, ("x", "weight", "bias", "y", "mean", "rstd")), (backward, ("x", "dy", "weight", "mean", "rstd", "dx", "dweight", "dbias")),
+                     (lookup, ("tokens", "table", "out")), (gradient, ("tokens", "dy", "dtable")), (schulz, ("g", "out"))):
+        for name in names:
+            with pytest.raises(ValueError, match=f"{name} has been freed"):
+                f(**{name: gone()})
