@@ -352,10 +352,12 @@ NEWTON_SCHULZ_QUINTIC = (3.4445, -4.7750, 2.0315)  # drives singular values into
 def newton_schulz(g: DeviceView, out: DeviceView, rows: int, cols: int, steps: int = 5, batch: int = 1, coefficients=NEWTON_SCHULZ_QUINTIC, eps: float = 1e-7) -> None:
     """Orthogonalises `batch` matrices [rows, cols] by `steps` Newton-Schulz products. coefficients: (a, b, c) of every
     step, or one such triple per step. g may be out."""
+    if not 1 <= steps <= 64:  # before there is a triple for each of them, and before the number becomes one of 32 bits
+        raise ValueError(f"{steps} Newton-Schulz steps (1 to 64 are taken)")
     triples = np.asarray(coefficients, dtype=np.float32)
     if triples.ndim == 1:
-        triples = np.tile(triples, (max(0, steps), 1))
-    if triples.shape != (max(0, steps), 3):
+        triples = np.tile(triples, (steps, 1))
+    if triples.shape != (steps, 3):
         raise ValueError(f"{steps} steps need three coefficients, or {steps} x 3; got an array of shape {triples.shape}")
     triples = np.ascontiguousarray(triples)
     n = batch * rows * cols

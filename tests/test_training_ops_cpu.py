@@ -146,3 +146,15 @@ def test_freed_buffers_are_refused_not_taken_as_left_out():
         for name in names:
             with pytest.raises(ValueError, match=f"{name} has been freed"):
                 f(**{name: gone()})
+
+
+@pytest.mark.parametrize("steps", [0, 65, 1 << 28, (1 << 32) + 5])
+def test_step_counts_are_looked_at_before_coefficients_are_laid_out(steps):
+    """One triple for each of 2^28 steps would take 3 GiB; 2^32 + 5 is 5 in the library's 32 bits."""
+    import tracemalloc
+
+    tracemalloc.start()
+    with pytest.raises(ValueError, match="1 to 64"):
+        runtime.newton_schulz(buf(1000), buf(1000), 8, 16, steps=steps)
+    assert tracemalloc.get_traced_memory()[1] < 1 << 20
+    tracemalloc.stop()
