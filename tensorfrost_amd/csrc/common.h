@@ -113,7 +113,8 @@ class CallGuard {
 inline bool words_overlap(const void* a, size_t a_words, const void* b, size_t b_words) {
 	if (!a || !b) return false;
 	const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
-	return pa < pb + b_words * 4 && pb < pa + a_words * 4;
+	// by distances: the end of a matrix of 2^31 - 1 x 2^31 - 1 words does not fit an address
+	return a_words && b_words && (pa < pb ? (pb - pa) / 4 < a_words : (pa - pb) / 4 < b_words);
 }
 
 // Checks the launch that was just issued.

@@ -158,3 +158,16 @@ def test_step_counts_are_looked_at_before_coefficients_are_laid_out(steps):
         runtime.newton_schulz(buf(1000), buf(1000), 8, 16, steps=steps)
     assert tracemalloc.get_traced_memory()[1] < 1 << 20
     tracemalloc.stop()
+
+
+@pytest.mark.parametrize("call", [
+    lambda high, most: embed(table=high, out=high + 64, vocab=most, cols=most, n=1), lambda high, most: embed_back(dtable=high, dy=high + 64, vocab=most, cols=most, n=1),
+    lambda high, most: norm(x=high, mean=high + 64, y=high, rows=most, cols=most), lambda high, most: norm_back(x=high, dw=high + 64, dx=None, rows=most, cols=most),
+])
+def test_overlaps_with_matrices_that_reach_past_the_last_address(call):
+    """(2^31 - 1)^2 words of 4 bytes from a usual device address on end beyond 2^64."""
+    assert call(0x7F0000000000, (1 << 31) - 1) == ARG and "overlap" in message()
+
+
+def test_arrays_without_elements_overlap_nothing():
+    assert norm_back(rows=0, x=at(6) + 4, dy=at(7) + 4, mean=at(6) + 8, rstd=at(7)) == STATE, message()
