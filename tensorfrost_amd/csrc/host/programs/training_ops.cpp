@@ -1,6 +1,6 @@
 // Programs around the operators of a training step that stand beside the dense layers' products. As in primitives.cpp, the
 // host part is what the reference's generator would emit for such a program and the kernels are primitive-backed.
-// Floating-point parameters are passed as the integer of their 32 bits.
+// Floating-point parameters are passed as the integer of their 32 bits; parameters that a program does not have are refused.
 //
 //   layer_norm            y, mean, rstd = f(x, weight, bias)                                  params: eps
 //   layer_norm_backward   dx, dweight, dbias = f(x, dy, weight, mean, rstd)
@@ -10,7 +10,10 @@
 //   embed_norm_dense      one step of embedding -> layer norm -> dense layer, forward and backward:
 //                         y, dtable, dweight, dbias, update = f(tokens, table, weight, bias, W, dy), update the orthogonalised
 //                         gradient of W                                                       params: eps, scale
+#include <cstdint>
 #include <cstring>
+#include <stdexcept>
+#include <string>
 
 #include "registry.h"
 
@@ -23,9 +26,17 @@ static int Bits(float v) {
 }
 static int Param(const std::vector<int64_t>& params, size_t i, int otherwise) { return i < params.size() ? (int)params[i] : otherwise; }
 
+// A program takes the same coefficients for all its steps, for one: triples of every step would be read as one triple.
+static void CheckParams(const char* program, const std::vector<int64_t>& params, size_t most) {
+	if (params.size() > most) throw std::runtime_error(std::string(program) + " takes at most " + std::to_string(most) + " parameters (got " + std::to_string(params.size()) + ")");
+	for (size_t i = 0; i < params.size(); i++)
+		if (params[i] < INT32_MIN || params[i] > (int64_t)UINT32_MAX) throw std::runtime_error(std::string(program) + ": parameter " + std::to_string(i) + " does not fit 32 bits");
+}
+
 static const float kLayerEps = 1e-5f, kNormEps = 1e-7f, kQuintic[3] = {3.4445f, -4.7750f, 2.0315f};
 
 static void BuildLayerNorm(Program* program, const std::vector<int64_t>& params) {
+	CheckParams("layer_norm", params, 1);
 	Kernel* norm = program->AddPrimitive("layer_norm_rows", 6, 3);
 	HostBuilder h(program);
 	V x = h.Input("x", {-1, -1}, TFType_Float);
@@ -40,7 +51,8 @@ static void BuildLayerNorm(Program* program, const std::vector<int64_t>& params)
 	h.Finish();
 }
 
-static void BuildLayerNormBackward(Program* program, const std::vector<int64_t>&) {
+static void BuildLayerNormBackward(Program* program, const std::vector<int64_t>& params) {
+	CheckParams("layer_norm_backward", params, 0);
 	Kernel* back = program->AddPrimitive("layer_norm_rows_backward", 8, 2);
 	HostBuilder h(program);
 	V x = h.Input("x", {-1, -1}, TFType_Float);
@@ -58,6 +70,7 @@ static void BuildLayerNormBackward(Program* program, const std::vector<int64_t>&
 }
 
 static void BuildEmbedding(Program* program, const std::vector<int64_t>& params) {
+	CheckParams("embedding", params, 1);
 	Kernel* lookup = program->AddPrimitive("embedding_rows", 3, 4);
 	HostBuilder h(program);
 	V tokens = h.Input("tokens", {-1}, TFType_Int);
@@ -70,6 +83,7 @@ static void BuildEmbedding(Program* program, const std::vector<int64_t>& params)
 }
 
 static void BuildEmbeddingBackward(Program* program, const std::vector<int64_t>& params) {
+	CheckParams("embedding_backward", params, 2);
 	if (params.empty() || params[0] < 1 || params[0] > 0x7FFFFFFF) throw std::runtime_error("embedding_backward needs the number of rows of the table as its first parameter");
 	Kernel* back = program->AddPrimitive("embedding_rows_backward", 3, 4);
 	HostBuilder h(program);
@@ -90,6 +104,7 @@ static std::vector<V> NewtonSchulzVariables(HostBuilder& h, V batch, V rows, V c
 }
 
 static void BuildNewtonSchulz(Program* program, const std::vector<int64_t>& params) {
+	CheckParams("newton_schulz", params, 5);
 	Kernel* schulz = program->AddPrimitive("newton_schulz", 2, 8);
 	HostBuilder h(program);
 	V g = h.Input("g", {-1, -1, -1}, TFType_Float);
@@ -101,6 +116,7 @@ static void BuildNewtonSchulz(Program* program, const std::vector<int64_t>& para
 }
 
 static void BuildEmbedNormDense(Program* program, const std::vector<int64_t>& params) {
+	CheckParams("embed_norm_dense", params, 2);
 	Kernel* lookup = program->AddPrimitive("embedding_rows", 3, 4);
 	Kernel* norm = program->AddPrimitive("layer_norm_rows", 6, 3);
 	Kernel* gemm_nn = program->AddPrimitive("sgemm_nn", 3, 3);
