@@ -414,9 +414,13 @@ static int embedding_sums(const uint32_t* keys, const uint32_t* order, const flo
 // their order by a ballot for every 64 tokens; a row with more than kFewAlone is cut into eight parts of neighbouring positions, one
 // per wave, added in their order at the end. us in the kernels, this one | the three launches below, which also wait for each
 // other for 6 us in all: 500 x 250 over 1009 rows 5.8 | 14.0, 37 x 560 over 22709 11 | 21, 1000 x 1024 over 100 9.0 | 14.6, 1551 x 86
-// over 6876 8.7 | 15.8, 2048 x 256 over 50000 13.6 | 24.9; the frequent rows decide where it ends: 2048 x 64 over 50 rows 22 | 16,
-// 2048 x 1024 over one 25 | 19, and 4096 x 100 over 100 34 | 20.
-constexpr uint32_t kFewPositions = 2048, kFewMostRows = 256;
+// over 6876 8.7 | 15.8, 2048 x 256 over 50000 13.6 | 24.9; and 4096 x 100 over 100 34 | 20.
+// A group owns eight rows or more and goes through those with many positions one after the other, so the table needs rows enough
+// to spread the positions: from kFewAnyTable positions on, one for kFewShare of them. us per call, tokens spread evenly:
+//   2048 x 256 over 8 rows 47 | 16, 50 rows 31 | 16, 64 rows 24 | 16, 100 rows 8 | 16 (with a few frequent ones 16 | 16)
+//   1024 x 256 over 8 rows 27 | 14, 32 rows 15 | 14, 64 rows 6 | 15;  512 x 256 over 8 rows 18 | 13, 16 rows 14 | 13;  256 x 256 over 8 rows 12 | 13
+// (tables of one or two rows have no such queue and give up a little of it: 512 x 256 over one row 8 | 12, over two 10 | 12)
+constexpr uint32_t kFewPositions = 2048, kFewMostRows = 256, kFewAnyTable = 384, kFewShare = 24;
 constexpr int kFewWaves = 8, kFewThreads = kFewWaves * 64, kFewAlone = 32;
 constexpr size_t kFewVocab = (size_t)1 << 30, kFewCols = 65535 * 64;  // a launch has fewer than 2^32 threads
 
@@ -551,7 +555,7 @@ extern "C" int tfhip_embedding_rows_backward_f32(const int32_t* tokens, const fl
 	TFHIP_HOLD_DEVICE();
 	State& s = state();
 	if (n == 0) return tfhip_fill_u32(dtable, 0u, vocab * cols);
-	if (n <= kFewPositions && vocab <= kFewVocab && cols <= kFewCols) {
+	if (n <= kFewPositions && (n <= kFewAnyTable || n <= vocab * kFewShare) && vocab <= kFewVocab && cols <= kFewCols) {
 		const RowShape r = row_shape(cols, dy, dtable);
 		// four groups a unit, with 8 to kFewMostRows rows each
 		const size_t stretches = (cols + 64 * r.vec - 1) / (64 * r.vec), wanted = (vocab * stretches + s.compute_units * 4 - 1) / (s.compute_units * 4);
