@@ -143,9 +143,15 @@ def prepare(case, seed):
 # ---- the framework's calls ------------------------------------------------------------------------
 
 def _own(s):
+    """The library works on a stream of its own, which torch's does not wait for and which does not wait for torch's. The first
+    call on a state waits until torch has filled it. The results are there, and the state may be dropped, once the whole
+    device (torch.cuda.synchronize) or the library's stream (rt.synchronize) has been waited for."""
     from tensorfrost_amd import runtime as rt
 
     rt.initialize(0)
+    if "filled" not in s:
+        torch.cuda.synchronize()
+        s["filled"] = True
     c = s["case"]
     b = {k: rt.DeviceBuffer.view(v.data_ptr(), v.numel()) for k, v in s.items() if isinstance(v, torch.Tensor)}
     if c["op"] == "ln_forward":
