@@ -96,6 +96,7 @@ _SIGNATURES = {
     "tfhip_embedding_rows_f32": [_vp, _vp, _vp, _sz, _sz, _sz, _f],
     "tfhip_embedding_rows_backward_f32": [_vp, _vp, _vp, _sz, _sz, _sz, _f],
     "tfhip_newton_schulz_f32": [_vp, _vp, _sz, _sz, _sz, _i, C.POINTER(_f), _f],
+    "tfhip_test_newton_schulz_tiles": [_sz, _sz, _sz, C.POINTER(_i), C.POINTER(C.c_uint)],
 }
 for _op in ("sum", "max", "min"):
     for _ax in ("rows", "cols"):

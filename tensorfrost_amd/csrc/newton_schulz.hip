@@ -947,9 +947,30 @@ static int newton_schulz_small(const float* g, float* out, size_t batch, size_t 
 	return TFHIP_OK;
 }
 
+static bool ns_fits_one_group(size_t shorter, size_t longer) { return shorter <= (size_t)kSmallRows && longer <= kSmallCols; }
+
+struct NsPlan {
+	int tile_half, tile_full;  // of the symmetric products and of the others
+	size_t mp, np;             // padded sides
+	size_t at_once;            // matrices, as many as a work space of 4 GiB holds, at least one
+};
+static NsPlan ns_plan(size_t batch, size_t m, size_t n) {
+	NsPlan p;
+	const size_t counted = batch < 256 ? batch : 256;
+	p.tile_half = ns_tile(m, m, true, counted);
+	p.tile_full = ns_tile(m, n, false, counted);
+	const size_t tile = p.tile_half > p.tile_full ? p.tile_half : p.tile_full;
+	p.mp = (m + tile - 1) / tile * tile;
+	p.np = (n + tile - 1) / tile * tile;
+	p.at_once = std::max<size_t>(1, ((size_t)4 << 30) / (16 * p.mp * p.np + 8 * p.mp * p.mp));
+	return p;
+}
+
 // `batch` matrices whose work space fits the arena together.
-static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps, int tile_half, int tile_full, size_t mp, size_t np) {
+static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps, const NsPlan& plan) {
 	State& s = state();
+	const int tile_half = plan.tile_half, tile_full = plan.tile_full;
+	const size_t mp = plan.mp, np = plan.np;
 	const bool transposed = rows > cols;
 	const size_t m = transposed ? cols : rows, n = transposed ? rows : cols, elements = rows * cols;
 	// a group takes four vectors a thread, or, where there are none, four elements (30 of 101 x 75: 9.6 -> 3.5 us, 1501 x 1003 6.6 -> 5.0)
@@ -1066,19 +1087,31 @@ extern "C" int tfhip_newton_schulz_f32(const float* g, float* out, size_t batch,
 	if (g != out && words_overlap(g, batch * rows * cols, out, batch * rows * cols)) return fail(TFHIP_ERR_ARG, "Newton-Schulz: g and out overlap without being the same");
 	TFHIP_REQUIRE_INIT();
 	TFHIP_HOLD_DEVICE();
-	if (shorter <= (size_t)kSmallRows && longer <= kSmallCols) return newton_schulz_small(g, out, batch, rows, cols, steps, coefficients, eps);
-	// As many matrices at a time as a work space of 4 GiB holds, at least one.
-	const size_t at_once = batch < 256 ? batch : 256;
-	const int tile_half = ns_tile(shorter, shorter, true, at_once), tile_full = ns_tile(shorter, longer, false, at_once);
-	const size_t tile = tile_half > tile_full ? tile_half : tile_full;
-	const size_t mp = (shorter + tile - 1) / tile * tile, np = (longer + tile - 1) / tile * tile;
-	size_t chunk = ((size_t)4 << 30) / (16 * mp * np + 8 * mp * mp);
-	if (chunk < 1) chunk = 1;
-	if (chunk > batch) chunk = batch;
-	for (size_t first = 0; first < batch; first += chunk) {
-		const size_t count = batch - first < chunk ? batch - first : chunk;
-		const int rc = newton_schulz(g + first * rows * cols, out + first * rows * cols, count, rows, cols, steps, coefficients, eps, tile_half, tile_full, mp, np);
+	if (ns_fits_one_group(shorter, longer)) return newton_schulz_small(g, out, batch, rows, cols, steps, coefficients, eps);
+	const NsPlan plan = ns_plan(batch, shorter, longer);
+	for (size_t first = 0; first < batch; first += plan.at_once) {
+		const size_t count = batch - first < plan.at_once ? batch - first : plan.at_once;
+		const int rc = newton_schulz(g + first * rows * cols, out + first * rows * cols, count, rows, cols, steps, coefficients, eps, plan);
 		if (rc) return rc;
 	}
+	return TFHIP_OK;
+}
+
+extern "C" int tfhip_test_newton_schulz_tiles(size_t batch, size_t rows, size_t cols, int* tiles, unsigned* cuts) {
+	TFHIP_REQUIRE_INIT();
+	const size_t shorter = rows < cols ? rows : cols, longer = rows < cols ? cols : rows;
+	if (!tiles || !cuts || batch == 0 || shorter == 0) return fail(TFHIP_ERR_ARG, "null pointer or empty batch passed to tfhip_test_newton_schulz_tiles");
+	tiles[0] = tiles[1] = 0;
+	cuts[0] = cuts[1] = cuts[2] = 1;
+	if (ns_fits_one_group(shorter, longer)) return TFHIP_OK;
+	const NsPlan plan = ns_plan(batch, shorter, longer);
+	const size_t count = batch < plan.at_once ? batch : plan.at_once;
+	const uint32_t blocks_m = (uint32_t)(plan.mp / kNsStep), blocks_n = (uint32_t)(plan.np / kNsStep);
+	size_t left;
+	tiles[0] = plan.tile_half;
+	tiles[1] = plan.tile_full;
+	cuts[0] = ns_cuts(ns_tiles(plan.mp, plan.mp, plan.tile_half, true), plan.tile_half, blocks_n, count, left);
+	cuts[1] = ns_cuts(ns_tiles(plan.mp, plan.mp, plan.tile_half, true), plan.tile_half, blocks_m, count, left);
+	cuts[2] = ns_cuts(ns_tiles(plan.mp, plan.np, plan.tile_full, false), plan.tile_full, blocks_m, count, left);
 	return TFHIP_OK;
 }
