@@ -12,8 +12,10 @@
 // on average, and the dropped lo lo is below 2^-22 of the product; in exchange the accumulator takes 16 terms a step instead of
 // 2, and the result after five steps is as far from the 64-bit one as that of fp32 products (1.3e-6 against 1.6e-6 of the norm at
 // 256 x 256). The scale is a power of two chosen on the host: the spectral norm of X is at most 1 at the start and at most
-// max |a s + b s^3 + c s^5| over the reachable s after a step, and no element exceeds it; the scale puts that bound at 2^15.
-// Elements below 2^-12 of the bound keep an absolute error of 2^-40 of it instead of a relative one.
+// max |a s + b s^3 + c s^5| over the reachable s after a step, and no element exceeds it; the scale puts that bound
+// between 2^14 and 2^15. hi is off by at most 2^-11 of the power of two below v, lo holds that to 2^-12 of itself, so the pair is
+// within 2^-23 of v, until lo reaches the fixed grid of 2^-24 of small fp16 numbers: elements below 2^-16 of the bound keep an
+// absolute error of 2^-39 of it instead.
 //
 // Layout. A row of a split matrix is a sequence of 128-byte blocks, 32 hi then the 32 lo of the same columns, so one
 // cache line holds a row's share of a step of 32 in k. Rows and columns are padded to whole tiles with zeros, which stay

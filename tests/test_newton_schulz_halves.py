@@ -141,3 +141,21 @@ def test_every_kernel_keeps_both_halves(rt, case):
         for k in {0, batch // 2, batch - 1}:
             want = expected(*pairs[k % len(pairs)])
             assert worst(got[k], want) <= bound(program, *sorted(shape)), (program, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 200), (200, 1), (40, 60), (1, 300), (300, 300), (1000, 1020)])
+def test_how_well_small_elements_are_held(rt, shape):
+    """X <- X. One row holds elements from 1 to 2^-45 of the norm, so that X has norm 1: each is held to 2^-23 of itself or, where that is more,
+    to 2^-39; the norm, the factor and the sum of the halves round by 2^-24 each."""
+    rng = np.random.default_rng(shape)
+    g = np.zeros(shape, np.float32)
+    line = g[:, 0] if shape[1] == 1 else g[shape[0] // 2]
+    line[:] = 2.0 ** -rng.uniform(0, 45, line.size) * rng.choice([-1.0, 1.0], line.size)
+    line[line.size // 3] = 3.0
+    gb, out = rt.DeviceBuffer.from_numpy(g), rt.DeviceBuffer(g.size)
+    rt.newton_schulz(gb, out, *shape, steps=1, coefficients=(1, 0, 0), eps=0.0)
+    want = g.astype(np.float64) / np.linalg.norm(g.astype(np.float64))
+    off = np.abs(out.numpy(np.float32, shape) - want)
+    assert (off <= np.maximum(2.0 ** -23 * np.abs(want), 2.0 ** -39) + 3 * 2.0 ** -24 * np.abs(want)).all()
+    assert off.max() > 0  # and not all of them better than that
