@@ -276,10 +276,11 @@ int tfhip_embedding_rows_backward_f32(const int32_t* tokens, const float* dy, fl
 /* Orthogonalises `batch` matrices [rows, cols] that follow each other: X = G / (|G|_F + eps), then `steps` times (1 to 64)
  * A = X X^T, X <- a X + (b A + c A^2) X with that step's three coefficients (host memory, 3 * steps finite floats: a, b, c
  * of the first step first); with rows > cols the same on the transposed matrix. Operands of the products keep 22 bits:
- * an element is held to 2^-23 of itself or, below 2^-16 of the bound on its matrix (1 for the first X), to 2^-39 of the
- * bound, so with |G|_F far below eps the small X of the first steps is known to 2^-39 only. A matrix of zeros stays zero;
- * one with an infinity or NaN comes out as NaN. g == out is allowed, any other overlap is refused. At most 32768 on the shorter side, 2^23 - 1 on the longer one,
- * 2^31 - 1 elements in a matrix and 65535 matrices; batch == 0 is a no-op. */
+ * an element is held to 2^-23 of itself or, below 2^-16 of the bound on its matrix, to 2^-39 of the bound. The bound of the
+ * first X is |G|_F / (|G|_F + eps), that of the next ones follows from the coefficients (a power of two above either; not
+ * less than 2^-100), so a G far below eps keeps its digits. A matrix of zeros stays zero; one with an infinity or NaN comes
+ * out as NaN. g == out is allowed, any other overlap is refused. At most 32768 on the shorter side, 2^23 - 1 on the longer
+ * one, 2^31 - 1 elements in a matrix and 65535 matrices; batch == 0 is a no-op. */
 int tfhip_newton_schulz_f32(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps);
 
 #ifdef __cplusplus

@@ -11,8 +11,8 @@
 // three fp16 products into one fp32 accumulator, hi hi + hi lo + lo hi. The pair keeps 22 bits, one less than fp32 keeps
 // on average, and the dropped lo lo is below 2^-22 of the product; in exchange the accumulator takes 16 terms a step instead of
 // 2, and the result after five steps is as far from the 64-bit one as that of fp32 products (1.3e-6 against 1.6e-6 of the norm at
-// 256 x 256). The scale is a power of two chosen on the host: the spectral norm of X is at most 1 at the start and at most
-// max |a s + b s^3 + c s^5| over the reachable s after a step, and no element exceeds it; the scale puts that bound
+// 256 x 256). The scale is a power of two from a bound on the spectral norm, which no element exceeds: of X it is 1 at the start (or, for a
+// G below eps, the power of two above |X|) and after a step max |a s + b s^3 + c s^5| over the reachable s; the scale puts that bound
 // between 2^14 and 2^15. hi is off by at most 2^-11 of the power of two below v, lo holds that to 2^-12 of itself, so the pair is
 // within 2^-23 of v, until lo reaches the fixed grid of 2^-24 of small fp16 numbers: elements below 2^-16 of the bound keep an
 // absolute error of 2^-39 of it instead.
@@ -78,6 +78,88 @@ __device__ __forceinline__ void store_split_tile(const float (&v)[16], uint32_t*
 	}
 }
 
+// ---- scales --------------------------------------------------------------------------------------
+
+// max |a s + b s^3 + c s^5| over s in [0, top]: at the end or where the derivative is 0.
+__host__ __device__ inline double largest_quintic(double a, double b, double c, double top) {
+	double best = 0.0;
+	auto look = [&](double t) {  // t = s^2
+		if (!(t >= 0.0 && t <= top * top)) return;
+		const double p = fabs((a + t * (b + t * c)) * sqrt(t));
+		if (!(p <= best)) best = p;
+	};
+	look(top * top);
+	const double u = a, v = 3.0 * b, w = 5.0 * c;  // u + v t + w t^2 = 0
+	if (w == 0.0) {
+		if (v != 0.0) look(-u / v);
+	} else if (v * v - 4.0 * u * w >= 0.0) {
+		const double root = sqrt(v * v - 4.0 * u * w);
+		look((-v + root) / (2.0 * w));
+		look((-v - root) / (2.0 * w));
+	}
+	return best;
+}
+
+// max |b t + c t^2| over t in [0, top], likewise.
+__host__ __device__ inline double largest_square(double b, double c, double top) {
+	const double end = fabs(top * (b + top * c)), t = c != 0.0 ? -b / (2.0 * c) : -1.0;
+	const double middle = t > 0.0 && t < top ? fabs(t * (b + t * c)) : 0.0;
+	return end > middle ? end : middle;
+}
+
+// The power of two that brings values of at most `bound` to at most 2^15.
+__host__ __device__ inline double scale_for(double bound) {
+	if (!(bound > 1e-30)) bound = 1e-30;
+	if (!(bound < 1e37)) bound = 1e37;
+	int e;
+	frexp(bound, &e);  // bound <= 2^e
+	return ldexp(1.0, 15 - e);
+}
+
+// What the products of a step are multiplied with on their way from one scale to another.
+struct NsFactors {
+	float gram;            // X X^T in A
+	float poly, poly_a;    // A^2 and A in B
+	float update, update_x;  // B X and X in the next X
+};
+
+// The scales of the split matrices, step by step.
+struct NsScales {
+	double bound;  // on the spectral norm of X
+	double next;   // the scale of X
+	__host__ __device__ explicit NsScales(double first) : bound(first), next(scale_for(first)) {}
+	__host__ __device__ NsFactors step(const float* abc, bool last) {
+		const double ca = abc[0], cb = abc[1], cc = abc[2], x = next;
+		// bounds that rounding does not cross
+		const double a = scale_for(bound * bound * 1.0001), b = scale_for(largest_square(cb, cc, bound * bound) * 1.0001);
+		bound = largest_quintic(ca, cb, cc, bound) * 1.0001;
+		next = last ? 1.0 : scale_for(bound);
+		return {(float)(a / (x * x)), (float)(cc * b / (a * a)), (float)(cb * b / a), (float)(next / (b * x)), (float)(ca * next / x)};
+	}
+};
+
+// The steps of a call: their coefficients, and their factors where |X| may be anything up to 1 at the start.
+struct NsSteps {
+	int count;
+	float coefficients[64][3];
+	NsFactors usual[64];
+};
+
+// What |X| = norm / (norm + eps) does not exceed: 1, or, where it is below a half, the next power of two, so that a gradient far below
+// eps keeps the digits of its small X. (|G| = 1e-13 with eps = 1e-7, 1000 x 1020, five steps: the result is off by 1.2e-7, with a bound
+// of 1 for all it was 1.1e-3.) Such a matrix has factors of its own, worked out by one thread of its group. The others pay for
+// factors in memory: 2 of 256 x 256 80.9 -> 81.5 us, 512 x 512 102.9 -> 104.1, 64 x 256 in one group 40.3 -> 40.8.
+__device__ inline double ns_first_bound(double norm, double eps) {
+	if (!(norm < eps)) return 1.0;
+	int e;
+	frexp(norm / (norm + eps), &e);
+	return ldexp(1.0, e);
+}
+__device__ inline void ns_own_factors(const NsSteps& steps, double first, NsFactors* to) {
+	NsScales scales(first);
+	for (int k = 0; k < steps.count; k++) to[k] = scales.step(steps.coefficients[k], k + 1 == steps.count);
+}
+
 // ---- the norm and the first split -----------------------------------------------------------------
 
 // Partial sums of squares, in 64 bits: the square of a large fp32 number does not fit fp32. `vec`: every matrix starts on
@@ -117,9 +199,10 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const float* __restrict__ 
 }
 
 // X and its transpose in split form from g. X is [mp, np] with mp, np padded; `transposed`: g is [n, m], else [m, n].
-// A wave per 32 x 32 tile, taken in turn; each group adds up the norm's parts for itself once.
+// A wave per 32 x 32 tile, taken in turn; each group adds up the norm's parts for itself once. The first group of a matrix writes
+// its factors, [matrix][step].
 __global__ __launch_bounds__(256) void ns_split_kernel(const float* __restrict__ g, const double* __restrict__ partial, unsigned parts, char* x, char* xt, size_t m, size_t n, size_t mp, size_t np,
-                                                       bool transposed, float eps, float scale) {
+                                                       bool transposed, float eps, NsFactors* __restrict__ factors, const NsSteps steps) {
 	__shared__ uint32_t lds[4][32 * 33];
 	__shared__ double red[4];
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -143,8 +226,16 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const float* __restrict__
 	sum = wave_reduce(sum, [](double a, double b) { return a + b; });
 	if (lane == 0) red[wave] = sum;
 	__syncthreads();
-	const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3])) + (double)eps;
-	const double r = !isfinite(norm) ? (double)nanf("") : norm > 0.0 ? (double)scale / norm : 0.0;
+	const double own = sqrt((red[0] + red[1]) + (red[2] + red[3])), norm = own + (double)eps, first = ns_first_bound(own, eps);
+	const double r = !isfinite(norm) ? (double)nanf("") : norm > 0.0 ? scale_for(first) / norm : 0.0;
+	if (blockIdx.x == 0) {
+		factors += matrix * steps.count;
+		if (first == 1.0) {
+			if ((int)threadIdx.x < steps.count) factors[threadIdx.x] = steps.usual[threadIdx.x];
+		} else if (threadIdx.x == 0) {
+			ns_own_factors(steps, first, factors);
+		}
+	}
 	while (tile < tiles) {
 		const size_t t0 = tile / tiles_n * 32, t1 = tile % tiles_n * 32;
 #pragma unroll
@@ -182,9 +273,21 @@ struct NsArgs {
 	uint32_t whole;   // tiles that one group each works on; the others are cut along k
 	uint32_t cuts;    // into so many parts
 	float4* partial;  // the parts' sums
-	float alpha;  // what an element of the accumulator is multiplied with
-	float beta;   // ... and an element of the addend
+	const NsFactors* factors;  // of this step of the first matrix
+	uint32_t steps;            // of a matrix
 };
+
+// What an element of the accumulator is multiplied with, and one of the addend. Read at the start of a kernel, where nothing waits for it.
+struct NsPair {
+	float alpha, beta;
+};
+template <int KIND>
+__device__ __forceinline__ NsPair pair_of(const NsArgs& g) {
+	const NsFactors* f = g.factors + (size_t)blockIdx.y * g.steps;
+	if (KIND == kNsGram) return {f->gram, 0.0f};
+	if (KIND == kNsPoly) return {f->poly, f->poly_a};
+	return {f->update, f->update_x};
+}
 
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
 
@@ -250,13 +353,13 @@ __device__ __forceinline__ void load_addend(const NsArgs& g, Addend& a, uint32_t
 
 // What a kind does with a finished 32 x 32 tile of P Q^T at (row0, col0), held by one wave in accumulator layout.
 template <int KIND>
-__device__ __forceinline__ void finish_tile(const NsArgs& g, float (&v)[16], const Addend& a, uint32_t row0, uint32_t col0, bool diagonal, uint32_t* corner) {
+__device__ __forceinline__ void finish_tile(const NsArgs& g, const NsPair& by, float (&v)[16], const Addend& a, uint32_t row0, uint32_t col0, bool diagonal, uint32_t* corner) {
 	const int lane = threadIdx.x & 63;
 #pragma unroll
-	for (int r = 0; r < 16; r++) v[r] *= g.alpha;
+	for (int r = 0; r < 16; r++) v[r] *= by.alpha;
 	if (KIND != kNsGram) {
 #pragma unroll
-		for (int r = 0; r < 16; r++) v[r] += g.beta * ((float)a.hi[r / 4][r % 4] + (float)a.lo[r / 4][r % 4]);
+		for (int r = 0; r < 16; r++) v[r] += by.beta * ((float)a.hi[r / 4][r % 4] + (float)a.lo[r / 4][r % 4]);
 	}
 	if (KIND == kNsLast) {
 		float* out = reinterpret_cast<float*>(reinterpret_cast<char*>(g.out) + blockIdx.y * g.batch_out);
@@ -297,6 +400,7 @@ __global__ __launch_bounds__(WP* WQ* KS * 64) void ns_product_kernel(const NsArg
 
 	const int lane = threadIdx.x & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const NsPair by = pair_of<KIND>(g);
 	uint32_t tp, tq;
 	uint32_t first = 0, steps = g.k_blocks;
 	const bool part = kCut && blockIdx.x >= g.whole;
@@ -432,7 +536,7 @@ __global__ __launch_bounds__(WP* WQ* KS * 64) void ns_product_kernel(const NsArg
 			}
 			Addend a;
 			if (KIND != kNsGram) load_addend(g, a, row0, col0);
-			finish_tile<KIND>(g, v, a, row0, col0, tp == tq, corner);
+			finish_tile<KIND>(g, by, v, a, row0, col0, tp == tq, corner);
 		}
 }
 
@@ -444,6 +548,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const NsArgs g) {
 	constexpr int SP = T / WP / 32, SQ = T / WQ / 32, kTiles = T / 32 * T / 32, kGroups = kTiles / 4;  // 32 x 32 tiles, groups for them
 	const int lane = threadIdx.x & 63, corner_of = threadIdx.x >> 6;
 	const uint32_t at = blockIdx.x / kGroups, sub = (blockIdx.x % kGroups) * 4 + corner_of;
+	const NsPair by = pair_of<KIND>(g);
 	uint32_t tp, tq;
 	place_of_tile<KIND>(g, g.whole + at, tp, tq);
 	const uint32_t wave = sub / (SP * SQ), i = sub / SQ % SP, j = sub % SQ;
@@ -464,7 +569,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const NsArgs g) {
 			v[4 * q + 2] += t.z;
 			v[4 * q + 3] += t.w;
 		}
-	finish_tile<KIND>(g, v, addend, row0, col0, tp == tq, corner[corner_of]);
+	finish_tile<KIND>(g, by, v, addend, row0, col0, tp == tq, corner[corner_of]);
 }
 
 // Few tiles: what counts is the way from the first load to the last store. A group of eight waves owns a 32 x 32 tile; each
@@ -482,6 +587,7 @@ __global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const 
 	__shared__ __attribute__((aligned(1024))) char lds[kDeepStages * kStage];
 	const int lane = threadIdx.x & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const NsPair by = pair_of<KIND>(g);
 	uint32_t tp, tq;
 	place_of_tile<KIND>(g, whole_tile_of_group(g), tp, tq);
 	const size_t stride = (size_t)g.k_blocks * kNsBlock;
@@ -563,7 +669,7 @@ __global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const 
 		v[4 * q + 2] = t.z;
 		v[4 * q + 3] = t.w;
 	}
-	finish_tile<KIND>(g, v, addend, tp * T, tq * T, tp == tq, reinterpret_cast<uint32_t*>(lds));
+	finish_tile<KIND>(g, by, v, addend, tp * T, tq * T, tp == tq, reinterpret_cast<uint32_t*>(lds));
 }
 
 // ---- small matrices: every step in one group ----------------------------------------------------------
@@ -585,11 +691,8 @@ struct NsSmallArgs {
 	float* out;
 	int m, n;  // rows and columns of X, m <= n
 	bool transposed;
-	float eps, scale;
-	int steps;
-	struct {
-		float gram, poly, poly_a, update, update_x;  // factors of A, A^2, A in B, B X, X
-	} step[64];
+	float eps;
+	NsSteps steps;
 };
 
 // Where piece c (16 bytes: 8 hi or, from c = 4 on, 8 lo) of block kb of a row lies. The sixteen pieces of two blocks are
@@ -602,6 +705,7 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 	constexpr int kRowX = NP * 4, kRowM = kSmallRows * 4;           // bytes of a row of X; of X^T and A
 	__shared__ __attribute__((aligned(256))) char lds[kA + kSmallRows * kSmallRows * 4];
 	__shared__ double red[kSmallWaves];
+	__shared__ NsFactors own_factors[64];  // of a matrix far below eps
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4;
 	const int m = a.m, n = a.n;
 	const float* g = a.g + (size_t)blockIdx.x * m * n;
@@ -626,8 +730,10 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 	sum = 0.0;
 #pragma unroll
 	for (int w = 0; w < kSmallWaves; w++) sum += red[w];
-	const double norm = sqrt(sum) + (double)a.eps;
-	const double factor = !isfinite(norm) ? (double)nanf("") : norm > 0.0 ? (double)a.scale / norm : 0.0;
+	const double own = sqrt(sum), norm = own + (double)a.eps, first = ns_first_bound(own, a.eps);
+	const double factor = !isfinite(norm) ? (double)nanf("") : norm > 0.0 ? scale_for(first) / norm : 0.0;
+	const bool usual = __builtin_amdgcn_readfirstlane(first == 1.0);
+	if (!usual && tid == 0) ns_own_factors(a.steps, first, own_factors);
 #pragma unroll
 	for (int t = 0; t < kTurns; t++) {
 		const int at = t * kSmallThreads + tid, r0 = at / (NP / 2) * 2, c0 = at % (NP / 2) * 2;
@@ -694,12 +800,18 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 
 	const int ti = (wave >> 2) * 16, tj = (wave & 3) * 16;  // this wave's tile of A and B
 	constexpr int kShare = NP / 32;                         // and its tiles of X and of X^T: 2 * 4 * NP / 16 among sixteen
-	for (int k = 0; k < a.steps; k++) {
+	auto uniform = [](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); };
+	for (int k = 0; k < a.steps.count; k++) {
+		NsFactors by;
+		if (usual)
+			by = a.steps.usual[k];
+		else
+			by = {uniform(own_factors[k].gram), uniform(own_factors[k].poly), uniform(own_factors[k].poly_a), uniform(own_factors[k].update), uniform(own_factors[k].update_x)};
 		forget();
 		floatx4 low = {0.0f, 0.0f, 0.0f, 0.0f}, high = low;
 #pragma unroll 4
 		for (int kb = 0; kb < NP / 32; kb++) multiply(low, high, read(kX, kRowX, ti, kb), read(kX, kRowX, tj, kb));
-		floatx4 r = a.step[k].gram * (low + high);
+		floatx4 r = by.gram * (low + high);
 		store(r, kA, kRowM, ti, tj);
 		__syncthreads();
 		// B in A's place
@@ -707,13 +819,13 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 #pragma unroll
 		for (int kb = 0; kb < 2; kb++) multiply(low, high, read(kA, kRowM, ti, kb), read(kA, kRowM, tj, kb));
 		r = low + high;
-		add(r, a.step[k].poly, a.step[k].poly_a, kA, kRowM, ti, tj);
+		add(r, by.poly, by.poly_a, kA, kRowM, ti, tj);
 		__syncthreads();
 		store(r, kA, kRowM, ti, tj);
 		__syncthreads();
 		// X: waves 0 .. 7 the tiles of B X (written to X^T), the others those of X^T B (written to X); a wave has one of the four
 		// rows of tiles of B and every second one of X^T
-		const bool last = k + 1 == a.steps;
+		const bool last = k + 1 == a.steps.count;
 		const int form = wave >> 3, mi = (wave & 3) * 16, n0 = (wave >> 2) & 1;
 		floatx4 x[kShare];
 		auto multiply_x = [&](auto which) {
@@ -733,9 +845,9 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 				}
 				x[i] = low + high;
 				if constexpr (kTurned)
-					add(x[i], a.step[k].update, a.step[k].update_x, kX, kRowX, ni, mi);
+					add(x[i], by.update, by.update_x, kX, kRowX, ni, mi);
 				else
-					add(x[i], a.step[k].update, a.step[k].update_x, kXt, kRowM, mi, ni);
+					add(x[i], by.update, by.update_x, kXt, kRowM, mi, ni);
 				forget();
 			}
 		};
@@ -774,56 +886,6 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 }
 
 // ---- the host's side --------------------------------------------------------------------------------
-
-// max |a s + b s^3 + c s^5| over s in [0, top]: at the end or where the derivative is 0.
-static double largest_quintic(double a, double b, double c, double top) {
-	double best = 0.0;
-	auto look = [&](double t) {  // t = s^2
-		if (!(t >= 0.0 && t <= top * top)) return;
-		const double p = fabs((a + t * (b + t * c)) * sqrt(t));
-		if (!(p <= best)) best = p;
-	};
-	look(top * top);
-	const double u = a, v = 3.0 * b, w = 5.0 * c;  // u + v t + w t^2 = 0
-	if (w == 0.0) {
-		if (v != 0.0) look(-u / v);
-	} else if (v * v - 4.0 * u * w >= 0.0) {
-		const double root = sqrt(v * v - 4.0 * u * w);
-		look((-v + root) / (2.0 * w));
-		look((-v - root) / (2.0 * w));
-	}
-	return best;
-}
-
-// max |b t + c t^2| over t in [0, top], likewise.
-static double largest_square(double b, double c, double top) {
-	const double end = fabs(top * (b + top * c)), t = c != 0.0 ? -b / (2.0 * c) : -1.0;
-	const double middle = t > 0.0 && t < top ? fabs(t * (b + t * c)) : 0.0;
-	return end > middle ? end : middle;
-}
-
-// The power of two that brings values of at most `bound` to at most 2^15.
-static double scale_for(double bound) {
-	if (!(bound > 1e-30)) bound = 1e-30;
-	if (!(bound < 1e37)) bound = 1e37;
-	int e;
-	frexp(bound, &e);  // bound <= 2^e
-	return ldexp(1.0, 15 - e);
-}
-
-// The scales of the split matrices, step by step: `next` is the one of X before the first step, then after the last one.
-struct NsScales {
-	double bound = 1.0;  // on the spectral norm of X
-	double x = 0.0, a = 0.0, b = 0.0, next = scale_for(1.0);
-	void step(double ca, double cb, double cc) {
-		x = next;
-		// bounds that rounding does not cross
-		a = scale_for(bound * bound * 1.0001);
-		b = scale_for(largest_square(cb, cc, bound * bound) * 1.0001);
-		bound = largest_quintic(ca, cb, cc, bound) * 1.0001;
-		next = scale_for(bound);
-	}
-};
 
 // The tile of a product whose result is m x n (half of m x m for the symmetric kinds). A larger tile reads less per product
 // but leaves compute units idle. The measured time of a step of 32 columns over all of the result is close to a line in the
@@ -917,7 +979,18 @@ static int ns_product(const NsArgs& args, int tile, size_t p_rows, size_t q_rows
 	return TFHIP_OK;
 }
 
-static int newton_schulz_small(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps) {
+static NsSteps ns_steps(int count, const float* coefficients) {
+	NsSteps s = {};
+	s.count = count;
+	NsScales scales(1.0);
+	for (int k = 0; k < count; k++) {
+		for (int i = 0; i < 3; i++) s.coefficients[k][i] = coefficients[3 * k + i];
+		s.usual[k] = scales.step(s.coefficients[k], k + 1 == count);
+	}
+	return s;
+}
+
+static int newton_schulz_small(const float* g, float* out, size_t batch, size_t rows, size_t cols, const NsSteps& steps, float eps) {
 	NsSmallArgs args = {};
 	args.g = g;
 	args.out = out;
@@ -926,18 +999,6 @@ static int newton_schulz_small(const float* g, float* out, size_t batch, size_t 
 	args.n = (int)(args.transposed ? rows : cols);
 	args.eps = eps;
 	args.steps = steps;
-	NsScales scales;
-	args.scale = (float)scales.next;
-	for (int k = 0; k < steps; k++) {
-		const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
-		scales.step(a, b, c);
-		const double after = k + 1 == steps ? 1.0 : scales.next;
-		args.step[k].gram = (float)(scales.a / (scales.x * scales.x));
-		args.step[k].poly = (float)(c * scales.b / (scales.a * scales.a));
-		args.step[k].poly_a = (float)(b * scales.b / scales.a);
-		args.step[k].update = (float)(after / (scales.b * scales.x));
-		args.step[k].update_x = (float)(a * after / scales.x);
-	}
 	const dim3 grid((unsigned)batch), block(kSmallThreads);
 	if (args.n <= 64)
 		hipLaunchKernelGGL(ns_small_kernel<64>, grid, block, 0, state().stream, args);
@@ -969,7 +1030,7 @@ static NsPlan ns_plan(size_t batch, size_t m, size_t n) {
 }
 
 // `batch` matrices whose work space fits the arena together.
-static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, size_t cols, int steps, const float* coefficients, float eps, const NsPlan& plan) {
+static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, size_t cols, const NsSteps& steps, float eps, const NsPlan& plan) {
 	State& s = state();
 	const int tile_half = plan.tile_half, tile_full = plan.tile_full;
 	const size_t mp = plan.mp, np = plan.np;
@@ -980,15 +1041,16 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 	const size_t share = vec ? 4096 : 1024, shares = elements / share;
 	const unsigned parts = (unsigned)(shares < 1 ? 1 : shares < 512 ? shares : 512);
 	auto align = [](size_t b) { return (b + 255) & ~size_t(255); };
-	const size_t norm_bytes = align(batch * parts * sizeof(double)), x_bytes = align(batch * mp * np * 4), a_bytes = align(batch * mp * mp * 4);
+	const size_t norm_bytes = align(batch * parts * sizeof(double)), factor_bytes = align(batch * steps.count * sizeof(NsFactors)), x_bytes = align(batch * mp * np * 4), a_bytes = align(batch * mp * mp * 4);
 	const uint32_t blocks_m = (uint32_t)(mp / kNsStep), blocks_n = (uint32_t)(np / kNsStep);
 	const size_t parts_bytes[3] = {ns_partial_bytes(mp, mp, tile_half, true, blocks_n, batch), ns_partial_bytes(mp, mp, tile_half, true, blocks_m, batch),
 	                               ns_partial_bytes(mp, np, tile_full, false, blocks_m, batch)};
 	const size_t partial_bytes = std::max({parts_bytes[0], parts_bytes[1], parts_bytes[2]});
-	char* base = (char*)scratch(norm_bytes + 4 * x_bytes + 2 * a_bytes + partial_bytes);
+	char* base = (char*)scratch(norm_bytes + factor_bytes + 4 * x_bytes + 2 * a_bytes + partial_bytes);
 	if (!base) return TFHIP_ERR_HIP;
 	double* partial = (double*)base;
-	char* x = base + norm_bytes;
+	NsFactors* factors = (NsFactors*)(base + norm_bytes);
+	char* x = base + norm_bytes + factor_bytes;
 	char* xt = x + x_bytes;
 	char* x_next = xt + x_bytes;
 	char* xt_next = x_next + x_bytes;
@@ -998,16 +1060,14 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 
 	hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)batch * parts), dim3(256), 0, s.stream, g, partial, elements, parts, vec);
 	TFHIP_CHECK_LAUNCH();
-	NsScales scales;
 	const size_t split_groups = (mp / 32 * (np / 32) + 3) / 4, most = (size_t)s.compute_units * 8;
 	hipLaunchKernelGGL(ns_split_kernel, dim3((unsigned)(split_groups < most ? split_groups : most), (unsigned)batch), dim3(256), 0, s.stream, g, (const double*)partial, parts, x, xt, m, n, mp, np, transposed, eps,
-	                   (float)scales.next);
+	                   factors, steps);
 	TFHIP_CHECK_LAUNCH();
-	for (int k = 0; k < steps; k++) {
-		const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
-		scales.step(a, b, c);
-		const double scale_x = scales.x, scale_a = scales.a, scale_b = scales.b, scale_next = scales.next;
+	for (int k = 0; k < steps.count; k++) {
 		NsArgs gram = {};
+		gram.factors = factors + k;
+		gram.steps = (uint32_t)steps.count;
 		gram.P = gram.Q = x;
 		gram.straight = gram.turned = A;
 		gram.straight_stride = gram.turned_stride = mp * 4;
@@ -1015,7 +1075,6 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 		gram.batch_out = mp * mp * 4;
 		gram.partial = products_partial;
 		gram.k_blocks = blocks_n;
-		gram.alpha = (float)(scale_a / (scale_x * scale_x));
 		int rc = ns_product<kNsGram>(gram, tile_half, mp, mp, batch);
 		if (rc) return rc;
 		NsArgs poly = gram;
@@ -1024,11 +1083,9 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 		poly.batch_p = poly.batch_q = poly.batch_addend = mp * mp * 4;
 		poly.addend_stride = mp * 4;
 		poly.k_blocks = blocks_m;
-		poly.alpha = (float)(c * scale_b / (scale_a * scale_a));
-		poly.beta = (float)(b * scale_b / scale_a);
 		rc = ns_product<kNsPoly>(poly, tile_half, mp, mp, batch);
 		if (rc) return rc;
-		const bool last = k + 1 == steps;
+		const bool last = k + 1 == steps.count;
 		const bool turn = last && transposed;  // the caller's rows are the columns of X
 		NsArgs update = {};
 		update.P = turn ? xt : B;
@@ -1039,14 +1096,14 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 		update.addend_stride = (turn ? np : mp) * 4;
 		update.batch_addend = mp * np * 4;
 		update.partial = products_partial;
+		update.factors = gram.factors;
+		update.steps = gram.steps;
 		update.k_blocks = blocks_m;
 		if (last) {
 			update.out = out;
 			update.out_rows = rows;
 			update.out_cols = cols;
 			update.batch_out = elements * sizeof(float);
-			update.alpha = (float)(1.0 / (scale_b * scale_x));
-			update.beta = (float)(a / scale_x);
 			rc = ns_product<kNsLast>(update, tile_full, turn ? np : mp, turn ? mp : np, batch);
 		} else {
 			update.straight = x_next;
@@ -1054,8 +1111,6 @@ static int newton_schulz(const float* g, float* out, size_t batch, size_t rows, 
 			update.straight_stride = np * 4;
 			update.turned_stride = mp * 4;
 			update.batch_out = mp * np * 4;
-			update.alpha = (float)(scale_next / (scale_b * scale_x));
-			update.beta = (float)(a * scale_next / scale_x);
 			rc = ns_product<kNsUpdate>(update, tile_full, mp, np, batch);
 		}
 		if (rc) return rc;
@@ -1089,11 +1144,12 @@ extern "C" int tfhip_newton_schulz_f32(const float* g, float* out, size_t batch,
 	if (g != out && words_overlap(g, batch * rows * cols, out, batch * rows * cols)) return fail(TFHIP_ERR_ARG, "Newton-Schulz: g and out overlap without being the same");
 	TFHIP_REQUIRE_INIT();
 	TFHIP_HOLD_DEVICE();
-	if (ns_fits_one_group(shorter, longer)) return newton_schulz_small(g, out, batch, rows, cols, steps, coefficients, eps);
+	const NsSteps taken = ns_steps(steps, coefficients);
+	if (ns_fits_one_group(shorter, longer)) return newton_schulz_small(g, out, batch, rows, cols, taken, eps);
 	const NsPlan plan = ns_plan(batch, shorter, longer);
 	for (size_t first = 0; first < batch; first += plan.at_once) {
 		const size_t count = batch - first < plan.at_once ? batch - first : plan.at_once;
-		const int rc = newton_schulz(g + first * rows * cols, out + first * rows * cols, count, rows, cols, steps, coefficients, eps, plan);
+		const int rc = newton_schulz(g + first * rows * cols, out + first * rows * cols, count, rows, cols, taken, eps, plan);
 		if (rc) return rc;
 	}
 	return TFHIP_OK;

@@ -35,14 +35,14 @@ def e(k):
     return 4 * 2.0 ** -22 + (k / 8 + 16) * 2.0 ** -24
 
 
-def bound(program, m, n):
-    x = 2 * R  # what X is off by, relative: the norm, the split
+def bound(program, m, n, r=R):
+    x = 2 * r  # what X is off by, relative: the norm, the split
     for a, b, c in program:
-        gram = e(n) + 2 * x + R
-        square = e(m) + 2 * gram + R
-        poly = b * gram + c * square + (b + c) * R
-        x = a * x + (b + c) * (e(m) + x) + poly + R
-    return x + 2 * R
+        gram = e(n) + 2 * x + r
+        square = e(m) + 2 * gram + r
+        poly = b * gram + c * square + (b + c) * r
+        x = a * x + (b + c) * (e(m) + x) + poly + r
+    return x + 2 * r
 
 
 def fraction(v):
