@@ -769,10 +769,14 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 		o.lo = *reinterpret_cast<const half8*>(p + (turn ^ 64));
 		return o;
 	};
-	auto multiply = [&](floatx4& low, floatx4& high, const Operand& p, const Operand& q) {
-		low = __builtin_amdgcn_mfma_f32_16x16x32_f16(p.lo, q.hi, low, 0, 0, 0);
+	// X and X^T are two copies that are carried on separately: the same element of both has to come out with the same bits. A difference
+	// between them, d, becomes a d in every step, however far X has converged (64 x 64, the quintic: no digit was left after 20
+	// steps). So an element is the same terms in the same order in both, whichever operand holds them: `turned` exchanges the two products
+	// with low halves along with the operands, and what is added afterwards leaves the compiler no choice of its roundings.
+	auto multiply = [&](floatx4& low, floatx4& high, const Operand& p, const Operand& q, auto turned) {
+		low = __builtin_amdgcn_mfma_f32_16x16x32_f16(turned ? p.hi : p.lo, turned ? q.lo : q.hi, low, 0, 0, 0);
 		high = __builtin_amdgcn_mfma_f32_16x16x32_f16(p.hi, q.hi, high, 0, 0, 0);
-		low = __builtin_amdgcn_mfma_f32_16x16x32_f16(p.hi, q.lo, low, 0, 0, 0);
+		low = __builtin_amdgcn_mfma_f32_16x16x32_f16(turned ? p.lo : p.hi, turned ? q.hi : q.lo, low, 0, 0, 0);
 	};
 	// where a lane's four rows of the tile (p0, q0) lie in D, which holds the result turned: D[q0 + lane's column][p0 + rows]
 	auto place = [&](int D, int d_bytes, int p0, int q0) {
@@ -784,7 +788,7 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 		const char* d = place(D, d_bytes, p0, q0);
 		const half4 hi = *reinterpret_cast<const half4*>(d), lo = *reinterpret_cast<const half4*>(reinterpret_cast<const char*>(lds) + ((d - lds) ^ 64));
 #pragma unroll
-		for (int i = 0; i < 4; i++) r[i] = alpha * r[i] + beta * ((float)hi[i] + (float)lo[i]);
+		for (int i = 0; i < 4; i++) r[i] = __builtin_fmaf(alpha, r[i], beta * ((float)hi[i] + (float)lo[i]));
 	};
 	auto store = [&](const floatx4& r, int D, int d_bytes, int p0, int q0) {
 		char* d = place(D, d_bytes, p0, q0);
@@ -810,14 +814,14 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 		forget();
 		floatx4 low = {0.0f, 0.0f, 0.0f, 0.0f}, high = low;
 #pragma unroll 4
-		for (int kb = 0; kb < NP / 32; kb++) multiply(low, high, read(kX, kRowX, ti, kb), read(kX, kRowX, tj, kb));
+		for (int kb = 0; kb < NP / 32; kb++) multiply(low, high, read(kX, kRowX, ti, kb), read(kX, kRowX, tj, kb), std::false_type());
 		floatx4 r = by.gram * (low + high);
 		store(r, kA, kRowM, ti, tj);
 		__syncthreads();
 		// B in A's place
 		low = high = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-		for (int kb = 0; kb < 2; kb++) multiply(low, high, read(kA, kRowM, ti, kb), read(kA, kRowM, tj, kb));
+		for (int kb = 0; kb < 2; kb++) multiply(low, high, read(kA, kRowM, ti, kb), read(kA, kRowM, tj, kb), std::false_type());
 		r = low + high;
 		add(r, by.poly, by.poly_a, kA, kRowM, ti, tj);
 		__syncthreads();
@@ -836,13 +840,8 @@ __global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const NsSmallAr
 				const int ni = (2 * i + n0) * 16;
 				low = high = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 				const Operand x0 = read(kXt, kRowM, ni, 0), x1 = read(kXt, kRowM, ni, 1);
-				if constexpr (kTurned) {
-					multiply(low, high, x0, b0);
-					multiply(low, high, x1, b1);
-				} else {
-					multiply(low, high, b0, x0);
-					multiply(low, high, b1, x1);
-				}
+				multiply(low, high, kTurned ? x0 : b0, kTurned ? b0 : x0, which);
+				multiply(low, high, kTurned ? x1 : b1, kTurned ? b1 : x1, which);
 				x[i] = low + high;
 				if constexpr (kTurned)
 					add(x[i], by.update, by.update_x, kX, kRowX, ni, mi);
