@@ -578,6 +578,9 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const NsArgs g) {
 // matrices: 5.1 us a product, about half of it the launch's own, against 6.3 with 64 x 64 tiles and one wave per quarter; with one step
 // asked for ahead instead of two 5.3, at 512 x 512 7.0 against 6.5. 64 x 64 tiles
 // in this form with four | eight waves: A of 1003 x 1501 22 | 16.4 us, X 20.5 | 24.4, where ns_product_kernel takes 15.8 and 19.2.)
+// Tiles of 32 are not cut along k between groups: A of a matrix with a short side takes some 0.43 us per 128 of its longer one
+// whatever the number of idle units (32 x 2^20 3.5 ms, 64 x 100000 0.3). The chains stay exact enough: 16 x 2^22, one step, 4.8e-7 against
+// 64 bits, fp32 products 4.4e-6.
 constexpr int kDeepWaves = 8, kDeepStages = 2;
 template <int KIND>
 __global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const NsArgs g) {
@@ -677,7 +680,7 @@ __global__ __launch_bounds__(kDeepWaves * 64) void ns_product_deep_kernel(const 
 // A matrix of at most 64 x 256 (the first and last layers of a small network) stays in the group memory of one compute unit
 // from its norm to its last product: X, its transpose and A (then B in its place) in split form, 2 * 64 * NP * 4 B + 16 KiB. One
 // launch instead of seventeen, which take 4 to 5 us each however little they compute. us in the kernels, this one | the seventeen:
-// one matrix of 64 x 64 17 | 65, 64 x 256 40 | 70, 256 x 3 38 | 67; 64 of 64 x 256 43 | 98, 1000 of them 203 | 490.
+// one matrix of 64 x 64 17 | 65, 64 x 256 41 | 70, 256 x 3 38 | 67; 64 of 64 x 256 43 | 98, 1000 of them 178 | 490.
 // Sixteen waves on 16 x 16 tiles (eight waves on 32 x 32 tiles: 21, 52 and, for the thousand, 268): the products are short, and
 // what takes the time between two barriers is the splitting of the results, some fifteen vector instructions an element, and the
 // group memory's latency; four waves a SIMD cover each other's.

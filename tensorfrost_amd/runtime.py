@@ -113,7 +113,7 @@ class DeviceBuffer(DeviceView):
 
     @staticmethod
     def view(ptr: int, n_words: int) -> DeviceView:
-        """A buffer over device memory that something else owns (a tensor of another library): never freed from here.
+        """A buffer over memory of the library's device that something else owns (a tensor of another library): never freed from here.
         The library's work runs on its own stream, so what fills or reads that memory elsewhere has to be waited for."""
         if not ptr or ptr & 3 or n_words <= 0:
             raise ValueError("a view needs a 4-byte aligned device address and at least one word")
